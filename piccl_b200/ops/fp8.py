@@ -1,0 +1,159 @@
+"""Linear layers in 8 bits: the quantiser and the products of src/ops/fp8_quant.cu and fp8_gemm.cu.
+
+A matrix in 8 bits (`Fp8`) is e4m3 values, rows filled with zeros to a multiple of 128, and one power of two for each block of 128
+values of a row: byte e stands for 2^(e - 127), the smallest for which the block's largest finite magnitude is at most 448.  Values that
+are not finite become NaN.  A product sums along the rows of both operands, so a matrix that two products sum over different
+dimensions is kept twice, the second time transposed; `square` gives both copies of a weight the same values.
+
+    w8, w8t = fp8.empty(N, K), fp8.empty(K, N)
+    fp8.quantize(w, w8, transposed=w8t, square=True)         # after each optimiser step
+    xt = fp8.empty(K, M)
+    fp8.linear(x, w8, y, bias=b, keep=xt)                    # y = x w^T + b; xt is what the backward pass needs of x, at a byte an element
+    fp8.linear_bwd(dy, xt, w8t, dx, dw)                      # dx = dy w, dw = dy^T x
+
+Sums are fp32 in the tensor cores; results are rounded once.  Calls launch on the current stream of their tensors' device, take workspace from PyTorch's
+allocator, and can be captured.  Empty results are left alone; a sum over nothing is zero (or the bias).
+"""
+from __future__ import annotations
+
+import ctypes as C
+from contextlib import nullcontext
+from typing import NamedTuple, Optional
+
+import torch
+
+from . import _bump, _s
+from .gemm_sm100 import _native, _ptr
+
+E4M3 = torch.float8_e4m3fn
+_QUANTIZE = [C.c_void_p, C.c_int] + [C.c_longlong] * 3 + [C.c_void_p] * 4 + [C.c_int, C.c_void_p]
+_GEMM = [C.c_void_p] * 6 + [C.c_int] * 3 + [C.c_longlong, C.c_int, C.c_void_p]
+
+
+class Fp8(NamedTuple):
+    """values: e4m3 [rows, columns up to a multiple of 128]; scales: uint8 [ceil(rows / 128), ceil(blocks / 4), 32, 4, 4], block k of row r at
+    [r // 128, k // 4, r % 32, r // 32 % 4, k % 4], the order in which the tensor cores take them."""
+    values: torch.Tensor
+    scales: torch.Tensor
+
+
+def empty(rows: int, cols: int, device="cuda") -> Fp8:
+    """Room for a matrix of `rows` by `cols`."""
+    blocks = (cols + 127) // 128
+    return Fp8(torch.empty(rows, blocks * 128, dtype=E4M3, device=device), torch.empty((rows + 127) // 128, (blocks + 3) // 4, 32, 4, 4, dtype=torch.uint8, device=device))
+
+
+def exponents(a: Fp8) -> torch.Tensor:
+    """The bytes of the scales as [rows, blocks]."""
+    s = a.scales
+    return s.permute(0, 3, 2, 1, 4).reshape(s.shape[0] * 128, s.shape[1] * 4)[:a.values.shape[0], :a.values.shape[1] // 128]
+
+
+def dequantize(a: Fp8, cols: Optional[int] = None) -> torch.Tensor:
+    """What the matrix stands for, in fp32 (its first `cols` columns)."""
+    v = torch.ldexp(a.values.float(), (exponents(a).to(torch.int32) - 127).repeat_interleave(128, 1))
+    return v if cols is None else v[:, :cols]
+
+
+def _on(device: torch.device):
+    return nullcontext() if torch._C._cuda_getDevice() == device.index else torch.cuda.device(device)
+
+
+def _check_fp8(a: Fp8, name: str, device) -> None:
+    v, s = a
+    if v.dim() != 2 or v.dtype != E4M3 or not v.is_contiguous() or v.shape[1] % 128:
+        raise ValueError(f"{name}: contiguous e4m3 values of whole blocks of 128 wanted, got {v.dtype} {tuple(v.shape)}")
+    if s.dtype != torch.uint8 or not s.is_contiguous() or tuple(s.shape) != ((v.shape[0] + 127) // 128, (v.shape[1] + 511) // 512, 32, 4, 4):
+        raise ValueError(f"{name}: the scales are not those of {tuple(v.shape)} values: {s.dtype} {tuple(s.shape)}")
+    if v.device != device or s.device != device:
+        raise ValueError(f"{name}: tensors of one CUDA device wanted")
+
+
+def _check_matrix(x: torch.Tensor, name: str, dtypes, contiguous: bool) -> None:
+    if x.dim() != 2 or x.dtype not in dtypes:
+        raise ValueError(f"{name}: a matrix of {' or '.join(str(t)[6:] for t in dtypes)} wanted, got {x.dtype} {tuple(x.shape)}")
+    if (contiguous and not x.is_contiguous()) or (x.shape[1] > 1 and x.stride(1) != 1) or (x.shape[0] > 1 and x.stride(0) < x.shape[1]):
+        raise ValueError(f"{name}: rows of values next to each other wanted, got strides {x.stride()}")
+    if not x.is_cuda:
+        raise ValueError(f"{name}: tensors of one CUDA device wanted")
+
+
+def _done(rc: int, what: str) -> None:
+    if rc != 0:
+        raise RuntimeError(f"{what} failed (code {rc})")
+    _bump()
+
+
+def quantize(x: torch.Tensor, out: Optional[Fp8], transposed: Optional[Fp8] = None, square: bool = False) -> None:
+    """x [R, C], bf16 or fp32, -> out, blocks along its rows (room for R x C), and transposed, blocks along its columns (room for C x R), either of which may be None.
+    square: one power of two for each 128 x 128 values."""
+    _check_matrix(x, "quantize", (torch.bfloat16, torch.float32), False)
+    if out is None and transposed is None:
+        raise ValueError("quantize: nothing to write")
+    R, Cc = x.shape
+    for a, rows, cols in ((out, R, Cc), (transposed, Cc, R)):
+        if a is not None:
+            _check_fp8(a, "quantize", x.device)
+            if tuple(a.values.shape) != (rows, (cols + 127) // 128 * 128):
+                raise ValueError(f"quantize: room for {rows} x {cols} wanted, got {tuple(a.values.shape)}")
+    if R == 0 or Cc == 0:
+        for a in (out, transposed):
+            if a is not None:
+                a.scales.fill_(1)
+        return
+    with _on(x.device):
+        q, t = out or (None, None), transposed or (None, None)
+        _done(_native("piccl_ops_fp8_quantize", _QUANTIZE)(x.data_ptr(), x.dtype == torch.float32, R, Cc, x.stride(0) if R > 1 else Cc, _ptr(q[0]), _ptr(q[1]), _ptr(t[0]), _ptr(t[1]), square, _s()),
+              "fp8 quantize")
+
+
+def product(a: Fp8, b: Fp8, out: torch.Tensor, bias: Optional[torch.Tensor] = None, _tile: int = 0) -> torch.Tensor:
+    """out [M, N] (bf16 or fp32) = a [M, K] b [N, K]^T + bias [N] (bf16)"""
+    _check_matrix(out, "product", (torch.bfloat16, torch.float32), True)
+    _check_fp8(a, "product", out.device)
+    _check_fp8(b, "product", out.device)
+    (M, K), Nn = a.values.shape, b.values.shape[0]
+    if b.values.shape[1] != K or tuple(out.shape) != (M, Nn):
+        raise ValueError(f"product: [{M}, {K}] and [{Nn}, {b.values.shape[1]}] do not give {tuple(out.shape)}")
+    if bias is not None and (bias.dtype != torch.bfloat16 or tuple(bias.shape) != (Nn,) or not bias.is_contiguous() or bias.device != out.device):
+        raise ValueError(f"product: a bias of {Nn} bf16 wanted, got {bias.dtype} {tuple(bias.shape)}")
+    if M == 0 or Nn == 0:
+        return out
+    if K == 0:
+        return out.zero_() if bias is None else out.copy_(bias.expand(M, Nn))
+    with _on(out.device):
+        _done(_native("piccl_ops_fp8_gemm", _GEMM)(a.values.data_ptr(), a.scales.data_ptr(), b.values.data_ptr(), b.scales.data_ptr(), _ptr(bias), out.data_ptr(), out.dtype == torch.float32, M, Nn, K,
+                                                   _tile, _s()), "fp8 product")
+    return out
+
+
+def linear(x: torch.Tensor, w: Fp8, out: torch.Tensor, bias: Optional[torch.Tensor] = None, keep: Optional[Fp8] = None) -> torch.Tensor:
+    """out [M, N] = x [M, K] w [N, K]^T + bias, x (bf16 or fp32) rounded to 8 bits on the way; keep: room for K x M, receives x along the tokens for linear_bwd."""
+    _check_matrix(x, "linear", (torch.bfloat16, torch.float32), False)
+    M, K = x.shape
+    if w.values.dim() != 2 or w.values.shape[1] != (K + 127) // 128 * 128:
+        raise ValueError(f"linear: weights of {K} columns wanted, got {tuple(w.values.shape)}")
+    q = empty(M, K, x.device)
+    quantize(x, q, keep)
+    return product(q, w, out, bias)
+
+
+def linear_bwd(dy: torch.Tensor, xt: Optional[Fp8], wt: Optional[Fp8], dx: Optional[torch.Tensor], dw: Optional[torch.Tensor]) -> None:
+    """dx [M, K] = dy [M, N] w, from the weights' transposed copy wt (K x N); dw [N, K] = dy^T x, from the input along the tokens xt (K x M).  dy (bf16 or fp32) is rounded to 8 bits, along
+    both dimensions in one pass.  dx or dw may be None."""
+    _check_matrix(dy, "linear_bwd", (torch.bfloat16, torch.float32), False)
+    if dx is None and dw is None:
+        return
+    if (dx is not None and wt is None) or (dw is not None and xt is None):
+        raise ValueError("linear_bwd: dx takes the transposed weights, dw the input along the tokens")
+    M, Nn = dy.shape
+    for a, n in ((wt if dx is not None else None, Nn), (xt if dw is not None else None, M)):
+        if a is not None and (a.values.dim() != 2 or a.values.shape[1] != (n + 127) // 128 * 128):
+            raise ValueError(f"linear_bwd: {n} columns wanted, got {tuple(a.values.shape)}")
+    q = empty(M, Nn, dy.device) if dx is not None else None
+    t = empty(Nn, M, dy.device) if dw is not None else None
+    quantize(dy, q, t)
+    if dx is not None:
+        product(q, wt, dx)
+    if dw is not None:
+        product(t, xt, dw)

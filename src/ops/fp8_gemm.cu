@@ -1,0 +1,315 @@
+// C[M, N] = A[M, K] B[N, K]^T + bias, operands in the 8-bit format of fp8.cuh, on CTA pairs: tcgen05.mma kind::mxf8f6f4, which multiplies by the scales of both
+// operands' blocks while it adds to fp32 accumulators in TMEM.
+//
+// The core is that of sm100_gemm_pair.cuh at a byte an element: a pair has 2 x 128 rows and TN columns, CTA v stages its own rows of A and half of the columns of B, k-blocks of
+// 128 (a 128-byte swizzled row each).  A block's scales: 512 bytes of A's 128 rows and of each 128 of B's columns hold four k-blocks; they come by TMA with every fourth k-block,
+// tcgen05.cp brings them into 4 columns of TMEM each, and the instruction names the byte of the word that is its block's.
+#include <cstring>
+#include <mutex>
+#include "../include/sm100_gemm_pair.cuh"
+#include "fp8.cuh"
+
+namespace piccl_ops {
+
+using namespace sm100;
+
+struct Fp8Args {
+  CUtensorMap ta, tb, sa, sb, tc;
+  const bf16* bias;
+  void* out;
+  int M, N, kb, k4, store_tma;       // k-blocks of 128, words of four of them
+  int* status;
+};
+
+constexpr int FP8_BM = 128, FP8_BK = 128, FP8_THREADS = 320;
+constexpr uint32_t kScaleCol = 496;        // TMEM columns: accumulators from 0 on, scales of A 4 from here, of B 8
+
+template <int TN, int STAGES>
+struct Fp8Smem {
+  static constexpr int A_BYTES = FP8_BM * FP8_BK, B_BYTES = TN / 2 * FP8_BK, STAGE = A_BYTES + B_BYTES;
+  static constexpr int NSF = TN > 128 ? 3 : 2, SF_BYTES = 512 * NSF;      // atoms of A's rows and of B's columns
+  static constexpr int SF_OFF = STAGES * STAGE, STAGING_OFF = (SF_OFF + STAGES * SF_BYTES + 1023) / 1024 * 1024;
+  static constexpr int BAR_OFF = STAGING_OFF + PAIR_EPI_WARPS * PAIR_STAGING;
+  static constexpr int TOTAL = BAR_OFF + (2 * STAGES + 4) * 8 + 16, DYNAMIC = TOTAL + 1024;
+  static_assert(DYNAMIC <= 232448, "more shared memory than a CTA can have");
+};
+
+// Instruction descriptor of kind::mxf8f6f4: e4m3 x e4m3, scales ue8m0, both operands K-major; the byte of the scale words comes on top
+__host__ __device__ constexpr uint32_t make_idesc_mxf8(uint32_t M, uint32_t N) { return ((N >> 3) << 17) | (1u << 23) | ((M >> 7) << 27); }
+__device__ __forceinline__ uint32_t idesc_byte(uint32_t b) { return b << 29 | b << 4; }
+// 32 rows of 16 bytes, unswizzled: groups of 8 rows are 128 bytes apart
+__device__ __forceinline__ uint64_t make_smem_desc_scales(const void* p) {
+  return (uint64_t)((smem_u32(p) & 0x3FFFFu) >> 4) | (uint64_t)(128u >> 4) << 32 | (uint64_t)1 << 46;
+}
+__device__ __forceinline__ void scales_to_tmem_pair(uint32_t taddr, uint64_t desc) {
+  asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+__device__ __forceinline__ void umma_mxf8_pair(uint32_t tmem_d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t sfa, uint32_t sfb, uint32_t accumulate) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\ttcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}\n"
+               ::"r"(tmem_d), "l"(da), "l"(db), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate) : "memory");
+}
+
+template <typename O> struct OutPiece;                     // 128 bytes of a row
+template <> struct OutPiece<bf16> {
+  static constexpr int COLS = 64;
+  static __device__ __forceinline__ void stage(uint8_t* row, int r, const float (&v)[64]) {
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      float f[8];
+#pragma unroll
+      for (int q = 0; q < 8; q++) f[q] = v[8 * j + q];
+      *reinterpret_cast<bf16x8*>(row + ((j ^ (r & 7)) << 4)) = pack8(f);
+    }
+  }
+};
+template <> struct OutPiece<float> {
+  static constexpr int COLS = 32;
+  static __device__ __forceinline__ void stage(uint8_t* row, int r, const float (&v)[32]) {
+#pragma unroll
+    for (int j = 0; j < 8; j++) *reinterpret_cast<float4*>(row + ((j ^ (r & 7)) << 4)) = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+  }
+};
+
+template <int TN, int STAGES, typename O>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FP8_THREADS, 1) fp8_pair_kernel(const __grid_constant__ Fp8Args a) {
+  typedef Fp8Smem<TN, STAGES> L;
+  constexpr int ACCS = TN <= 128 ? 2 : 1;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  __shared__ int s_abort;
+  uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* const full = reinterpret_cast<uint64_t*>(smem + L::BAR_OFF);
+  uint64_t *const empty = full + STAGES, *const tmem_full = empty + STAGES, *const tmem_empty = tmem_full + 2;
+  uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(tmem_empty + 2);
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31, v = (int)cluster_ctarank();
+  const int num_m = (a.M + 255) / 256, num_n = (a.N + TN - 1) / TN, num_tiles = num_m * num_n, first = blockIdx.x >> 1, stride = gridDim.x >> 1;
+  auto tile = [&](int t, int& m_blk, int& n_blk) {         // bands of 16 row tiles, as in gemm_sm100.cu
+    const int per_band = 16 * num_n, band = t / per_band, within = t % per_band, rows = min(16, num_m - band * 16);
+    m_blk = 2 * (band * 16 + within % rows) + v; n_blk = within / rows;
+  };
+  if (threadIdx.x == 0) {
+    s_abort = 0;
+    for (int s = 0; s < STAGES; s++) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+    for (int i = 0; i < 2; i++) { mbar_init(&tmem_full[i], 1); mbar_init(&tmem_empty[i], 2 * PAIR_EPI_WARPS); }
+    fence_barrier_init();
+  }
+  if (warp == 1) { tmem_alloc_pair(tmem_slot, 512); tmem_relinquish_pair(); }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  pdl_begin();
+
+  if (warp == 0) {
+    const bool issuer = elect_one();
+    int stage = 0; uint32_t phase = 0;
+    for (int t = first; t < num_tiles && !*(volatile int*)&s_abort; t += stride) {
+      int m_blk, n_blk; tile(t, m_blk, n_blk);
+      bool ok = true;
+      for (int kb = 0; kb < a.kb; kb++) {
+        if (!mbar_wait(&empty[stage], phase ^ 1, &s_abort, kPairWaitLimitNs)) { if (issuer) atomicExch(a.status, 11); ok = false; break; }
+        uint8_t *const pa = smem + stage * L::STAGE, *const pb = pa + L::A_BYTES, *const ps = smem + L::SF_OFF + stage * L::SF_BYTES;
+        if (issuer) {
+          const bool scales = (kb & 3) == 0;
+          if (v == 0) mbar_arrive_expect_tx(&full[stage], 2 * (L::STAGE + (scales ? L::SF_BYTES : 0)));
+          tma_load_2d_pair(pa, &a.ta, kb * FP8_BK, m_blk * FP8_BM, &full[stage]);
+          tma_load_2d_pair(pb, &a.tb, kb * FP8_BK, n_blk * TN + v * (TN / 2), &full[stage]);
+          if (scales) {
+            const int w = kb >> 2;
+            tma_load_2d_pair(ps, &a.sa, 0, m_blk * a.k4 + w, &full[stage]);
+            tma_load_2d_pair(ps + 512, &a.sb, 0, (n_blk * TN >> 7) * a.k4 + w, &full[stage]);
+            if (TN > 128) tma_load_2d_pair(ps + 1024, &a.sb, 0, ((n_blk * TN >> 7) + 1) * a.k4 + w, &full[stage]);
+          }
+        }
+        __syncwarp();
+        if (++stage == STAGES) { stage = 0; phase ^= 1; }
+      }
+      if (!ok) break;
+    }
+  } else if (warp == 1) {
+    if (v == 0) {
+      const bool issuer = elect_one();
+      constexpr uint32_t idesc = make_idesc_mxf8(256, TN);
+      const uint64_t da0 = make_smem_desc_k128(smem), db0 = make_smem_desc_k128(smem + L::A_BYTES), ds0 = make_smem_desc_scales(smem + L::SF_OFF);
+      const uint32_t sfa = tmem + kScaleCol, sfb = sfa + 4;
+      int stage = 0; uint32_t phase = 0; int local = 0;
+      for (int t = first; t < num_tiles && !*(volatile int*)&s_abort; t += stride, local++) {
+        int m_blk, n_blk; tile(t, m_blk, n_blk);
+        const int acc = local % ACCS; const uint32_t acc_phase = (local / ACCS) & 1;
+        if (!mbar_wait(&tmem_empty[acc], acc_phase ^ 1, &s_abort, kPairWaitLimitNs)) { if (issuer) atomicExch(a.status, 12); break; }
+        tc_fence_after();
+        const uint32_t d = tmem + acc * TN;
+        const uint32_t sfb_t = sfb + (TN == 64 ? 2 * (n_blk & 1) : 0);
+        bool ok = true;
+        for (int kb = 0; kb < a.kb; kb++) {
+          if (!mbar_wait(&full[stage], phase, &s_abort, kPairWaitLimitNs)) { if (issuer) atomicExch(a.status, 13); ok = false; break; }
+          tc_fence_after();
+          const uint64_t da = desc_advance(da0, stage * L::STAGE), db = desc_advance(db0, stage * L::STAGE);
+          if (issuer) {
+            if ((kb & 3) == 0) {
+              const uint64_t ds = desc_advance(ds0, stage * L::SF_BYTES);
+              scales_to_tmem_pair(sfa, ds);
+              scales_to_tmem_pair(sfb, desc_advance(ds, 512));
+              if (TN > 128) scales_to_tmem_pair(sfb + 4, desc_advance(ds, 1024));
+            }
+#pragma unroll
+            for (int k = 0; k < FP8_BK / 32; k++) umma_mxf8_pair(d, desc_advance(da, k * 32), desc_advance(db, k * 32), idesc | idesc_byte(kb & 3), sfa, sfb_t, kb != 0 || k != 0);
+            umma_commit_pair(&empty[stage]);
+          }
+          __syncwarp();
+          if (++stage == STAGES) { stage = 0; phase ^= 1; }
+        }
+        if (!ok) break;
+        if (issuer) umma_commit_pair(&tmem_full[acc]);
+        __syncwarp();
+      }
+    }
+  } else {
+    typedef OutPiece<O> P;
+    constexpr int PIECES = TN / P::COLS, PER = PIECES >= 2 ? PIECES / 2 : 1;
+    EpiCtx e;
+    e.quarter = warp & 3; e.half = (warp - 2) >> 2; e.lane = lane;
+    e.staging = smem + L::STAGING_OFF + (warp - 2) * PAIR_STAGING;
+    int local = 0;
+    for (int t = first; t < num_tiles; t += stride, local++) {
+      int m_blk, n_blk; tile(t, m_blk, n_blk);
+      const int acc = local % ACCS; const uint32_t acc_phase = (local / ACCS) & 1;
+      e.tmem = tmem + ((uint32_t)(e.quarter * 32) << 16) + acc * TN;
+      if (!mbar_wait(&tmem_full[acc], acc_phase, &s_abort, kPairWaitLimitNs)) { atomicExch(a.status, 14); break; }
+      tc_fence_after();
+      const int row0 = m_blk * FP8_BM + e.quarter * 32;
+      if (row0 < a.M && (PIECES >= 2 || e.half == 0)) {
+#pragma unroll 1
+        for (int pc = e.half * PER; pc < e.half * PER + PER; pc++) {
+          const int col = n_blk * TN + pc * P::COLS;
+          if (col >= a.N) break;
+          float x[P::COLS];
+#pragma unroll
+          for (int q = 0; q < P::COLS / 32; q++) {
+            uint32_t r[32];
+            tmem_ld_32x32(e.tmem + pc * P::COLS + 32 * q, r);
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 32; i++) x[32 * q + i] = __uint_as_float(r[i]);
+          }
+          if (a.bias) {
+#pragma unroll
+            for (int i = 0; i < P::COLS; i++) x[i] += __bfloat162float(a.bias[min(col + i, a.N - 1)]);
+          }
+          epi_staging_free(e);
+          P::stage(e.staging + lane * 128, lane, x);
+          if (a.store_tma) {
+            fence_proxy_async();
+            __syncwarp();
+            epi_ship(e, &a.tc, col, row0);
+          } else {                                         // rows that do not start on 16 bytes: a row at a time
+            __syncwarp();
+            O* const out = static_cast<O*>(a.out);
+            for (int r = 0; r < 32 && row0 + r < a.M; r++)
+#pragma unroll
+              for (int c = lane; c < P::COLS; c += 32)
+                if (col + c < a.N) {
+                  const int byte = c * (int)sizeof(O);
+                  out[(size_t)(row0 + r) * a.N + col + c] = *reinterpret_cast<const O*>(e.staging + r * 128 + (((byte >> 4) ^ (r & 7)) << 4) + (byte & 15));
+                }
+            __syncwarp();
+          }
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_leader(&tmem_empty[acc]);
+    }
+  }
+  // the ending of gemm_pair_persistent: nobody leaves while the other CTA may still touch its shared memory or barriers
+  tc_fence_before();
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  if (warp >= 2 && lane == 0) bulk_wait_read_all();
+  __syncwarp();
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  if (*(volatile int*)&s_abort) {
+    const unsigned long long t0 = gtime_ns();
+    while (gtime_ns() - t0 < 2000000ull) __nanosleep(1000);
+    __syncthreads();
+  }
+  if (warp == 1) { tc_fence_after(); tmem_dealloc_pair(tmem, 512); }
+}
+
+// ------------------------------------------------------------------ host
+// [rows, cols] of a type of esz bytes, boxes of box_rows x box_cols, rows of 128 bytes swizzled
+static bool fp8_map(CUtensorMap* out, CUtensorMapDataType type, int esz, const void* base, uint64_t rows, uint64_t cols, uint32_t box_rows, uint32_t box_cols, bool swizzle) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return false;
+  cuuint64_t dims[2] = {cols, rows}, strides[1] = {cols * esz};
+  cuuint32_t box[2] = {box_cols, box_rows}, estr[2] = {1, 1};
+  return fn(out, type, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+typedef void (*Fp8Fn)(Fp8Args);
+struct Fp8Variant { int tn, f32; Fp8Fn fn; int smem; };
+static const Fp8Variant g_fp8[] = {
+  {256, 0, fp8_pair_kernel<256, 5, bf16>, Fp8Smem<256, 5>::DYNAMIC}, {128, 0, fp8_pair_kernel<128, 7, bf16>, Fp8Smem<128, 7>::DYNAMIC}, {64, 0, fp8_pair_kernel<64, 8, bf16>, Fp8Smem<64, 8>::DYNAMIC},
+  {256, 1, fp8_pair_kernel<256, 5, float>, Fp8Smem<256, 5>::DYNAMIC}, {128, 1, fp8_pair_kernel<128, 7, float>, Fp8Smem<128, 7>::DYNAMIC}, {64, 1, fp8_pair_kernel<64, 8, float>, Fp8Smem<64, 8>::DYNAMIC},
+};
+static int g_fp8_pairs[64] = {0};
+
+static int fp8_ready(int dev) {
+  static std::mutex mu;
+  std::lock_guard<std::mutex> l(mu);
+  if (g_fp8_pairs[dev]) return 0;
+  for (const Fp8Variant& v : g_fp8) if (cudaFuncSetAttribute((const void*)v.fn, cudaFuncAttributeMaxDynamicSharedMemorySize, v.smem) != cudaSuccess) return -4;
+  int sms = 148; cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(sms / 2 * 2); cfg.blockDim = dim3(FP8_THREADS); cfg.dynamicSmemBytes = g_fp8[0].smem;
+  cudaLaunchAttribute at; memset(&at, 0, sizeof at);
+  at.id = cudaLaunchAttributeClusterDimension; at.val.clusterDim.x = 2; at.val.clusterDim.y = 1; at.val.clusterDim.z = 1;
+  cfg.attrs = &at; cfg.numAttrs = 1;
+  int active = 0, n = sms / 2;
+  if (cudaOccupancyMaxActiveClusters(&active, g_fp8[0].fn, &cfg) == cudaSuccess && active > 0) n = active < n ? active : n;
+  else cudaGetLastError();
+  g_fp8_pairs[dev] = n;
+  return 0;
+}
+
+}  // namespace piccl_ops
+
+using namespace piccl_ops;
+
+extern "C" {
+
+// a [M, K], b [N, K], K a multiple of 128, with their scales; out [M, N] bf16 or fp32, rows next to each other; bias [N] bf16 or null.  force_tn: 0, or the tile's width.
+int piccl_ops_fp8_gemm(const void* a, const void* sa, const void* b, const void* sb, const void* bias, void* out, int f32, int M, int N, long long K, int force_tn, void* stream) {
+  if (M <= 0 || N <= 0 || K <= 0 || K % 128 || K > 0x7fffff00ll || M > 0x7fffff00 || N > 0x7fffff00) return -1;
+  for (const void* p : {a, sa, b, sb}) if (!p || (reinterpret_cast<uintptr_t>(p) & 15)) return -2;
+  if (!out || (reinterpret_cast<uintptr_t>(out) & (f32 ? 3 : 1)) || (reinterpret_cast<uintptr_t>(bias) & 1)) return -2;
+  int dev = 0; cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64) return -6;
+  const int rc = fp8_ready(dev); if (rc) return rc;
+  const long row_tiles = (M + 255) / 256;
+  const Fp8Variant* v = nullptr; double best = 0;
+  for (const Fp8Variant& c : g_fp8) {
+    if (c.f32 != (f32 != 0) || (force_tn && c.tn != force_tn)) continue;
+    const long tiles = row_tiles * ((N + c.tn - 1) / c.tn);
+    const double cost = (double)((tiles + g_fp8_pairs[dev] - 1) / g_fp8_pairs[dev]) * (c.tn == 256 ? 136 : c.tn == 128 ? 84 : 70);
+    if (!v || cost < best) { v = &c; best = cost; }
+  }
+  if (!v) return -1;
+  Fp8Args g;
+  memset(&g, 0, sizeof g);
+  g.M = M; g.N = N; g.kb = (int)(K / 128); g.k4 = (g.kb + 3) / 4; g.bias = (const bf16*)bias; g.out = out;
+  const int esz = f32 ? 4 : 2;
+  g.store_tma = (size_t)N * esz % 16 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0;
+  const auto u8 = CU_TENSOR_MAP_DATA_TYPE_UINT8, u32 = CU_TENSOR_MAP_DATA_TYPE_UINT32;
+  if (!fp8_map(&g.ta, u8, 1, a, M, K, FP8_BM, FP8_BK, true) || !fp8_map(&g.tb, u8, 1, b, N, K, v->tn / 2, FP8_BK, true) ||
+      !fp8_map(&g.sa, u32, 4, sa, (uint64_t)((M + 127) / 128) * g.k4, 128, 1, 128, false) || !fp8_map(&g.sb, u32, 4, sb, (uint64_t)((N + 127) / 128) * g.k4, 128, 1, 128, false)) return -3;
+  if (g.store_tma && !fp8_map(&g.tc, f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, esz, out, M, N, 32, 128 / esz, true)) return -3;
+  g.status = status_word(STATUS_GEMM);
+  if (!g.status) return -7;
+  const long tiles = row_tiles * ((N + v->tn - 1) / v->tn);
+  const int pairs = (int)(tiles < g_fp8_pairs[dev] ? tiles : g_fp8_pairs[dev]);
+  return launch_pdl(v->fn, dim3(2 * pairs), dim3(FP8_THREADS), v->smem, (cudaStream_t)stream, g) == cudaSuccess ? 0 : -5;
+}
+
+}  // extern "C"
