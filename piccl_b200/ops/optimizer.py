@@ -1,0 +1,118 @@
+"""AdamW over many tensors in one launch (src/ops/adamw_many.cu), moments in fp32 or in 8 bits.
+
+    opt = AdamW(params, grads, masters, bits=8, decay=[p.dim() > 1 for p in params])
+    opt.step(lr, b1, b2, eps, wd)
+
+Parameters are bf16 with an fp32 master each, or fp32 with none; gradients are bf16 or fp32; tensors are contiguous, of any size and at any address.
+`decay` says which of them decay (all, by default).  The number of steps done lives on the device (`step_dev`, advanced by each step), so that a
+step can be captured into a CUDA graph and replayed; `gscale` multiplies the gradients, and may be a device tensor (a clipping factor that nobody reads back).
+
+Moments are the optimiser's own: `m` and `v`, flat, each tensor from a multiple of 128 elements on (`places`).  In 8 bits they are e4m3 values with
+a power of two for each block of 128 (`m_scales`, `v_scales`: byte e stands for 2^(e - 127)), v as its root, and are rounded stochastically, by bits that
+depend on the element's place, the step and `seed` alone: 2.02 bytes a parameter in place of 8.  Values that are not finite are held as NaN.
+
+One step at a time: steps of one optimiser on several streams need the order that any two writers of the same tensors need.
+"""
+from __future__ import annotations
+
+import ctypes as C
+from typing import Optional, Sequence, Union
+
+import torch
+
+from . import _bump, _s
+from .fp8 import E4M3, _on
+from .gemm_sm100 import _native, _ptr
+
+_DECAY, _P_F32, _G_F32, _WORDS = 1, 2, 4, 8
+_STEP = [C.c_void_p, C.c_int, C.c_longlong, C.c_int] + [C.c_void_p] * 4 + [C.c_float, C.c_double, C.c_double] + [C.c_float] * 3 + [C.c_void_p] * 3 + [C.c_uint, C.c_void_p]
+
+
+class _Tensor(C.Structure):          # AdamTensor of src/ops/adamw_many.cu
+    _fields_ = [("p", C.c_void_p), ("master", C.c_void_p), ("g", C.c_void_p), ("n", C.c_longlong), ("block", C.c_longlong), ("flags", C.c_int), ("pad", C.c_int)]
+
+
+class AdamW:
+    def __init__(self, params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], masters: Optional[Sequence[torch.Tensor]] = None, bits: int = 32,
+                 decay: Optional[Sequence[bool]] = None, seed: int = 0):
+        if bits not in (8, 32):
+            raise ValueError(f"AdamW: moments of 8 or 32 bits, not {bits}")
+        params, grads = list(params), list(grads)
+        masters = [None] * len(params) if masters is None else list(masters)
+        decay = [True] * len(params) if decay is None else list(decay)
+        if not params or not len(params) == len(grads) == len(masters) == len(decay):
+            raise ValueError(f"AdamW: {len(params)} parameters, {len(grads)} gradients, {len(masters)} masters, {len(decay)} decays")
+        self.device = params[0].device
+        for p, w in zip(params, masters):
+            if p.dtype not in (torch.bfloat16, torch.float32) or (p.dtype == torch.float32) != (w is None):
+                raise ValueError("AdamW: parameters are bf16 with a master or fp32 without")
+            if w is not None and (w.dtype != torch.float32 or w.numel() != p.numel()):
+                raise ValueError(f"AdamW: an fp32 master of {p.numel()} elements wanted, got {w.dtype} {tuple(w.shape)}")
+            for t in (p,) if w is None else (p, w):
+                if not t.is_contiguous() or not t.is_cuda or t.device != self.device:
+                    raise ValueError("AdamW: contiguous tensors of one CUDA device wanted")
+        self.params, self.masters, self.decay, self.bits, self.seed = params, masters, [bool(d) for d in decay], bits, int(seed) & 0xFFFFFFFF
+        self.places, block = [], 0                    # (first element in m and v, elements) of each tensor
+        for p in params:
+            self.places.append((block * 128, p.numel()))
+            block += (p.numel() + 127) // 128
+        self.blocks = block
+        zeros = lambda n, dtype: torch.zeros(n, dtype=dtype, device=self.device)  # noqa: E731
+        kind = E4M3 if bits == 8 else torch.float32
+        self.m, self.v = zeros(block * 128, kind), zeros(block * 128, kind)
+        self.m_scales, self.v_scales = (torch.ones(block, dtype=torch.uint8, device=self.device) for _ in range(2)) if bits == 8 else (None, None)
+        self.step_dev, self._ticket = zeros(1, torch.int32), zeros(1, torch.int32)
+        self._table = None
+        self.set_grads(grads)
+
+    def set_grads(self, grads: Sequence[torch.Tensor]) -> None:
+        """Other tensors to take the gradients from, from the next step on (a copy of addresses to the device; not within a capture)."""
+        grads = list(grads)
+        if len(grads) != len(self.params):
+            raise ValueError(f"AdamW: {len(self.params)} gradients wanted, got {len(grads)}")
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("AdamW: gradients cannot be exchanged within a capture")
+        records = []
+        for p, w, g, d, (first, n) in zip(self.params, self.masters, grads, self.decay, self.places):
+            if g.dtype not in (torch.bfloat16, torch.float32) or g.numel() != n or not g.is_contiguous() or g.device != self.device:
+                raise ValueError(f"AdamW: a contiguous gradient of {n} elements, bf16 or fp32, on {self.device} wanted, got {g.dtype} {tuple(g.shape)} on {g.device}")
+            if n == 0:
+                continue
+            flags = _DECAY * d | _P_F32 * (w is None) | _G_F32 * (g.dtype == torch.float32)
+            if all(t is None or t.data_ptr() % (4 * t.element_size()) == 0 for t in (p, w, g)):
+                flags |= _WORDS
+            records.append(_Tensor(p.data_ptr(), 0 if w is None else w.data_ptr(), g.data_ptr(), n, first // 128, flags, 0))
+        self.grads, self._count = grads, len(records)
+        raw = torch.frombuffer(bytearray((_Tensor * max(1, len(records)))(*records)), dtype=torch.uint8)
+        if self._table is None:
+            self._table = raw.to(self.device)
+        else:
+            self._table.copy_(raw)                    # in place: captured steps read it, and steps before on this stream have
+
+    def step(self, lr: float, b1: float = 0.9, b2: float = 0.95, eps: float = 1e-8, wd: float = 0.1, gscale: Union[float, torch.Tensor] = 1.0) -> None:
+        """One step from the gradients as they are now."""
+        if not (0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0):
+            raise ValueError(f"AdamW: decay rates of the moments are in [0, 1), not {b1} and {b2}")
+        dev = None
+        if isinstance(gscale, torch.Tensor):
+            if gscale.dtype != torch.float32 or gscale.numel() != 1 or gscale.device != self.device:
+                raise ValueError("AdamW: gscale is a number or one fp32 value on the device of the parameters")
+            gscale, dev = 1.0, gscale
+        with _on(self.device):
+            rc = _native("piccl_ops_adamw_many", _STEP)(self._table.data_ptr(), self._count, self.blocks, self.bits == 8, self.m.data_ptr(), self.v.data_ptr(), _ptr(self.m_scales),
+                                                        _ptr(self.v_scales), lr, b1, b2, eps, wd, gscale, _ptr(dev), self.step_dev.data_ptr(), self._ticket.data_ptr(), self.seed, _s())
+        if rc != 0:
+            raise RuntimeError(f"adamw_many failed (code {rc})")
+        _bump()
+
+    def moments(self, i: int) -> tuple[torch.Tensor, torch.Tensor]:
+        """m and v of tensor i as they are held, in fp32."""
+        o, n = self.places[i]
+        if self.bits == 32:
+            return self.m[o:o + n].clone(), self.v[o:o + n].clone()
+        out = []
+        for values, scales in ((self.m, self.m_scales), (self.v, self.v_scales)):
+            k = (n + 127) // 128
+            x = torch.ldexp(values[o:o + k * 128].float().view(k, 128), scales[o // 128:o // 128 + k, None].to(torch.int32) - 127)
+            out.append(x.reshape(-1)[:n])
+        return out[0], out[1] * out[1]

@@ -17,6 +17,7 @@ __device__ __forceinline__ uint32_t scale_byte(uint32_t amax_bits) {
   return e < 1 ? 1u : (uint32_t)e;
 }
 __device__ __forceinline__ float scale_inverse(uint32_t byte) { return __uint_as_float((254u - byte) << 23); }      // 2^(127 - byte), always a normal number
+__device__ __forceinline__ float scale_value(uint32_t byte) { return __uint_as_float(byte << 23); }                   // 2^(byte - 127)
 __device__ __forceinline__ size_t scale_at(long long row, int block, int blocks4) {
   return (((size_t)(row >> 7) * blocks4 + (block >> 2)) * 32 + (row & 31)) * 16 + ((row >> 5) & 3) * 4 + (block & 3);
 }
