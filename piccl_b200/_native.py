@@ -107,6 +107,22 @@ def fastcall():
         return _libs["fastcall"]
 
 
+def tensorcall():
+    """The module that takes tensors for the 8-bit layers (src/python/tensorcall.cc); None where it could not be built for want of Python's headers."""
+    with _lock:
+        if "tensorcall" not in _libs:
+            import torch  # noqa: F401
+            from . import build as _build
+            if not (_LIB_DIR / "_tensorcall.so").exists() and _build.python_headers() is None:
+                _libs["tensorcall"] = None
+                return None
+            _ensure_built("libpiccl_ops.so")
+            spec = importlib.util.spec_from_file_location("_tensorcall", _ensure_built("_tensorcall.so"))
+            _libs["tensorcall"] = importlib.util.module_from_spec(spec)
+            spec.loader.exec_module(_libs["tensorcall"])
+        return _libs["tensorcall"]
+
+
 def address(function) -> int:
     """Where a function of a library is."""
     return C.cast(function, C.c_void_p).value

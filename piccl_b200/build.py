@@ -4,6 +4,7 @@
   piccl_b200/lib/libpiccl_ops.so model kernels (tcgen05 GEMM, layer norm, cross entropy, AdamW, ...)
   piccl_b200/lib/libpiccl_model.so native training step (launches the kernels of libpiccl_ops.so; attention partly through ATen)
   piccl_b200/lib/_fastcall.so    calls with lists of tensors for the Python front end (where Python's headers are installed)
+  piccl_b200/lib/_tensorcall.so  the 8-bit layers' calls, which take tensors (likewise)
   piccl_b200/lib/piccl_sched     schedule dump / validation command line tool
   piccl_b200/lib/coll_bench      OSU-style collective benchmark (fork per GPU, no MPI)
   piccl_b200/lib/loggp_bench     PRTT measurements between two GPUs (input of tools/loggp_param)
@@ -82,7 +83,9 @@ def targets() -> dict[str, dict]:
         },
     }
     if inc := python_headers():
-        plan["_fastcall.so"] = {"src": _sources("python/*.cc"), "flags": [f"-I{inc}"], "link": ["-shared", "-cudart", "none"]}
+        plan["_fastcall.so"] = {"src": _sources("python/fastcall.cc"), "flags": [f"-I{inc}"], "link": ["-shared", "-cudart", "none"]}
+        model = plan["libpiccl_model.so"]
+        plan["_tensorcall.so"] = {"src": _sources("python/tensorcall.cc"), "flags": [f"-I{inc}", *model["flags"]], "link": [*model["link"], "-ltorch_python"]}
     return plan
 
 

@@ -22,12 +22,24 @@ from typing import NamedTuple, Optional
 
 import torch
 
+from .. import _native as N
 from . import _bump, _s
 from .gemm_sm100 import _native, _ptr
 
 E4M3 = torch.float8_e4m3fn
 _QUANTIZE = [C.c_void_p, C.c_int] + [C.c_longlong] * 3 + [C.c_void_p] * 4 + [C.c_int, C.c_void_p]
 _GEMM = [C.c_void_p] * 6 + [C.c_int] * 3 + [C.c_longlong, C.c_int, C.c_void_p]
+_SCRATCH = [C.c_void_p, C.c_int, C.c_longlong, C.c_int, C.c_longlong, C.c_int]
+_LINEAR = [C.c_void_p, C.c_int, C.c_longlong] + [C.c_void_p] * 4 + [C.c_int] + [C.c_void_p] * 4 + [C.c_int] * 2 + [C.c_longlong, C.c_void_p]
+_fast = None
+
+
+def _native_calls():
+    """The calls as one native function each (src/python/tensorcall.cc), or False where Python's headers are missing: a layer through ctypes is 23 us of host time, through it 5."""
+    global _fast
+    if _fast is None:
+        _fast = N.tensorcall() or False
+    return _fast
 
 
 class Fp8(NamedTuple):
@@ -87,6 +99,10 @@ def _done(rc: int, what: str) -> None:
 def quantize(x: torch.Tensor, out: Optional[Fp8], transposed: Optional[Fp8] = None, square: bool = False) -> None:
     """x [R, C], bf16 or fp32, -> out, blocks along its rows (room for R x C), and transposed, blocks along its columns (room for C x R), either of which may be None.
     square: one power of two for each 128 x 128 values."""
+    fast = _native_calls()
+    if fast and (n := fast.quantize(x, out, transposed, square)):
+        _bump(n)
+        return
     _check_matrix(x, "quantize", (torch.bfloat16, torch.float32), False)
     if out is None and transposed is None:
         raise ValueError("quantize: nothing to write")
@@ -107,16 +123,25 @@ def quantize(x: torch.Tensor, out: Optional[Fp8], transposed: Optional[Fp8] = No
               "fp8 quantize")
 
 
-def product(a: Fp8, b: Fp8, out: torch.Tensor, bias: Optional[torch.Tensor] = None, _tile: int = 0) -> torch.Tensor:
-    """out [M, N] (bf16 or fp32) = a [M, K] b [N, K]^T + bias [N] (bf16)"""
+def _check_product(a: tuple, b: Fp8, out: torch.Tensor, bias) -> None:
     _check_matrix(out, "product", (torch.bfloat16, torch.float32), True)
-    _check_fp8(a, "product", out.device)
     _check_fp8(b, "product", out.device)
-    (M, K), Nn = a.values.shape, b.values.shape[0]
+    (M, K), Nn = a, b.values.shape[0]
     if b.values.shape[1] != K or tuple(out.shape) != (M, Nn):
         raise ValueError(f"product: [{M}, {K}] and [{Nn}, {b.values.shape[1]}] do not give {tuple(out.shape)}")
     if bias is not None and (bias.dtype != torch.bfloat16 or tuple(bias.shape) != (Nn,) or not bias.is_contiguous() or bias.device != out.device):
         raise ValueError(f"product: a bias of {Nn} bf16 wanted, got {bias.dtype} {tuple(bias.shape)}")
+
+
+def product(a: Fp8, b: Fp8, out: torch.Tensor, bias: Optional[torch.Tensor] = None, _tile: int = 0) -> torch.Tensor:
+    """out [M, N] (bf16 or fp32) = a [M, K] b [N, K]^T + bias [N] (bf16)"""
+    fast = _native_calls()
+    if fast and not _tile and (n := fast.product(a, b, out, bias)):
+        _bump(n)
+        return out
+    _check_fp8(a, "product", out.device)
+    _check_product(tuple(a.values.shape), b, out, bias)
+    (M, K), Nn = a.values.shape, b.values.shape[0]
     if M == 0 or Nn == 0:
         return out
     if K == 0:
@@ -129,10 +154,25 @@ def product(a: Fp8, b: Fp8, out: torch.Tensor, bias: Optional[torch.Tensor] = No
 
 def linear(x: torch.Tensor, w: Fp8, out: torch.Tensor, bias: Optional[torch.Tensor] = None, keep: Optional[Fp8] = None) -> torch.Tensor:
     """out [M, N] = x [M, K] w [N, K]^T + bias, x (bf16 or fp32) rounded to 8 bits on the way; keep: room for K x M, receives x along the tokens for linear_bwd."""
+    fast = _native_calls()
+    if fast and (n := fast.linear(x, w, out, bias, keep)):
+        _bump(n)
+        return out
     _check_matrix(x, "linear", (torch.bfloat16, torch.float32), False)
     M, K = x.shape
     if w.values.dim() != 2 or w.values.shape[1] != (K + 127) // 128 * 128:
         raise ValueError(f"linear: weights of {K} columns wanted, got {tuple(w.values.shape)}")
+    if keep is None and M and K and M <= 64 and not _native("piccl_ops_fp8_linear_scratch", _SCRATCH)(x.data_ptr(), x.dtype == torch.float32, x.stride(0) if M > 1 else K, M, K, False):
+        _check_product((M, w.values.shape[1]), w, out, bias)
+        if out.device != x.device:
+            raise ValueError("linear: tensors of one CUDA device wanted")
+        if out.numel() == 0:
+            return out
+        with _on(x.device):
+            rc = _native("piccl_ops_fp8_linear", _LINEAR)(x.data_ptr(), False, x.stride(0) if M > 1 else K, w.values.data_ptr(), w.scales.data_ptr(), _ptr(bias), out.data_ptr(),
+                                                          out.dtype == torch.float32, None, None, None, None, M, out.shape[1], K, _s())
+            _done(min(rc, 0), "fp8 linear")
+        return out
     q = empty(M, K, x.device)
     quantize(x, q, keep)
     return product(q, w, out, bias)
@@ -141,6 +181,10 @@ def linear(x: torch.Tensor, w: Fp8, out: torch.Tensor, bias: Optional[torch.Tens
 def linear_bwd(dy: torch.Tensor, xt: Optional[Fp8], wt: Optional[Fp8], dx: Optional[torch.Tensor], dw: Optional[torch.Tensor]) -> None:
     """dx [M, K] = dy [M, N] w, from the weights' transposed copy wt (K x N); dw [N, K] = dy^T x, from the input along the tokens xt (K x M).  dy (bf16 or fp32) is rounded to 8 bits, along
     both dimensions in one pass.  dx or dw may be None."""
+    fast = _native_calls()
+    if fast and (n := fast.linear_bwd(dy, xt, wt, dx, dw)):
+        _bump(n)
+        return
     _check_matrix(dy, "linear_bwd", (torch.bfloat16, torch.float32), False)
     if dx is None and dw is None:
         return

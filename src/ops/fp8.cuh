@@ -10,6 +10,9 @@
 
 namespace piccl_ops {
 
+// fp8_few.cu: products of at most 64 rows
+int fp8_few(const bf16* x, long long stride, const void* a, const void* sa, const void* b, const void* sb, const void* bias, void* out, int f32, int M, int N, int K, int splits, void* stream);
+
 // bits of |x|, 0 for what is not finite
 __device__ __forceinline__ uint32_t finite_bits(float x) { const uint32_t u = __float_as_uint(x) & 0x7fffffffu; return u < 0x7f800000u ? u : 0u; }
 __device__ __forceinline__ uint32_t scale_byte(uint32_t amax_bits) {
@@ -26,6 +29,61 @@ __device__ __forceinline__ uint32_t e4m3_pair(float lo, float hi) {
   uint16_t r;
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
   return r;
+}
+
+// Eight values of a row as they lie in memory, and their magnitudes' bits: bf16 in pairs, 16 bits each, fp32 one by one.  A maximum over these counts values that are not finite; where it says
+// that there are some (a bit pattern from `kInf` on), the maximum is taken again without them.
+__device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) { return __vmaxu2(a, b); }
+template <typename T> struct Eight;
+template <> struct Eight<bf16> {
+  static constexpr int W = 4;                       // words
+  uint32_t w[4];
+  __device__ __forceinline__ void load(const bf16* p) { const uint4 u = *reinterpret_cast<const uint4*>(p); w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w; }
+  __device__ __forceinline__ void set(int e, const bf16* p) { w[e >> 1] |= (uint32_t)*reinterpret_cast<const uint16_t*>(p) << (16 * (e & 1)); }
+  __device__ __forceinline__ float at(int e) const { return __uint_as_float(e & 1 ? w[e >> 1] & 0xffff0000u : w[e >> 1] << 16); }
+  static __device__ __forceinline__ uint32_t magnitude(uint32_t w) { return w & 0x7fff7fffu; }
+  static __device__ __forceinline__ uint32_t most(uint32_t a, uint32_t b) { return max_u16x2(a, b); }
+  static __device__ __forceinline__ uint32_t bits(uint32_t m, int half) { return half ? m & 0xffff0000u : m << 16; }      // of fp32
+};
+template <> struct Eight<float> {
+  static constexpr int W = 8;
+  uint32_t w[8];
+  __device__ __forceinline__ void load(const float* p) {
+    const uint4 a = reinterpret_cast<const uint4*>(p)[0], b = reinterpret_cast<const uint4*>(p)[1];
+    w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w; w[4] = b.x; w[5] = b.y; w[6] = b.z; w[7] = b.w;
+  }
+  __device__ __forceinline__ void set(int e, const float* p) { w[e] = __float_as_uint(*p); }
+  __device__ __forceinline__ float at(int e) const { return __uint_as_float(w[e]); }
+  static __device__ __forceinline__ uint32_t magnitude(uint32_t w) { return w & 0x7fffffffu; }
+  static __device__ __forceinline__ uint32_t most(uint32_t a, uint32_t b) { return max(a, b); }
+  static __device__ __forceinline__ uint32_t bits(uint32_t m, int) { return m; }
+};
+constexpr uint32_t kInf = 0x7f800000u;
+
+// the largest magnitude of eight values, as bits of fp32
+template <typename T> __device__ __forceinline__ uint32_t top8(const Eight<T>& x) {
+  uint32_t m = Eight<T>::magnitude(x.w[0]);
+#pragma unroll
+  for (int i = 1; i < Eight<T>::W; i++) m = Eight<T>::most(m, Eight<T>::magnitude(x.w[i]));
+  return sizeof(T) == 2 ? max(m & 0xffff0000u, m << 16) : m;
+}
+template <typename T> __device__ __forceinline__ uint32_t finite_top8(const Eight<T>& x) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int e = 0; e < 8; e++) m = max(m, finite_bits(x.at(e)));
+  return m;
+}
+// satfinite takes infinities for 448: they are turned into NaN before, where there are any
+__device__ __forceinline__ float nan_of_inf(float x) { return (__float_as_uint(x) & 0x7fffffffu) >= kInf ? __uint_as_float(0x7fffffffu) : x; }
+__device__ __forceinline__ uint32_t pack4(float a, float b, float c, float d, float f) {
+  float x, y, z, w;
+  unpack2(mul2(pack2(a, b), both2(f)), x, y);
+  unpack2(mul2(pack2(c, d), both2(f)), z, w);
+  return e4m3_pair(x, y) | e4m3_pair(z, w) << 16;
+}
+template <typename T> __device__ __forceinline__ uint2 pack_row(const Eight<T>& x, float f, bool odd) {      // odd: values that are not finite are among these
+  if (odd) return make_uint2(pack4(nan_of_inf(x.at(0)), nan_of_inf(x.at(1)), nan_of_inf(x.at(2)), nan_of_inf(x.at(3)), f), pack4(nan_of_inf(x.at(4)), nan_of_inf(x.at(5)), nan_of_inf(x.at(6)), nan_of_inf(x.at(7)), f));
+  return make_uint2(pack4(x.at(0), x.at(1), x.at(2), x.at(3), f), pack4(x.at(4), x.at(5), x.at(6), x.at(7), f));
 }
 
 }  // namespace piccl_ops

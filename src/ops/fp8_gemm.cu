@@ -8,6 +8,8 @@
 #include <mutex>
 #include "../include/sm100_gemm_pair.cuh"
 #include "fp8.cuh"
+#include "fp8_mma.cuh"
+#include "piccl_ops.h"
 
 namespace piccl_ops {
 
@@ -33,21 +35,6 @@ struct Fp8Smem {
   static constexpr int TOTAL = BAR_OFF + (2 * STAGES + 4) * 8 + 16, DYNAMIC = TOTAL + 1024;
   static_assert(DYNAMIC <= 232448, "more shared memory than a CTA can have");
 };
-
-// Instruction descriptor of kind::mxf8f6f4: e4m3 x e4m3, scales ue8m0, both operands K-major; the byte of the scale words comes on top
-__host__ __device__ constexpr uint32_t make_idesc_mxf8(uint32_t M, uint32_t N) { return ((N >> 3) << 17) | (1u << 23) | ((M >> 7) << 27); }
-__device__ __forceinline__ uint32_t idesc_byte(uint32_t b) { return b << 29 | b << 4; }
-// 32 rows of 16 bytes, unswizzled: groups of 8 rows are 128 bytes apart
-__device__ __forceinline__ uint64_t make_smem_desc_scales(const void* p) {
-  return (uint64_t)((smem_u32(p) & 0x3FFFFu) >> 4) | (uint64_t)(128u >> 4) << 32 | (uint64_t)1 << 46;
-}
-__device__ __forceinline__ void scales_to_tmem_pair(uint32_t taddr, uint64_t desc) {
-  asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
-}
-__device__ __forceinline__ void umma_mxf8_pair(uint32_t tmem_d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t sfa, uint32_t sfb, uint32_t accumulate) {
-  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\ttcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}\n"
-               ::"r"(tmem_d), "l"(da), "l"(db), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate) : "memory");
-}
 
 template <typename O> struct OutPiece;                     // 128 bytes of a row
 template <> struct OutPiece<bf16> {
@@ -153,7 +140,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FP8_THREADS, 1) fp8_
               if (TN > 128) scales_to_tmem_pair(sfb + 4, desc_advance(ds, 1024));
             }
 #pragma unroll
-            for (int k = 0; k < FP8_BK / 32; k++) umma_mxf8_pair(d, desc_advance(da, k * 32), desc_advance(db, k * 32), idesc | idesc_byte(kb & 3), sfa, sfb_t, kb != 0 || k != 0);
+            for (int k = 0; k < FP8_BK / 32; k++) umma_mxf8_pair(d, desc_advance(da, k * 32), desc_advance(db, k * 32), idesc | idesc_bytes(kb & 3, kb & 3), sfa, sfb_t, kb != 0 || k != 0);
             umma_commit_pair(&empty[stage]);
           }
           __syncwarp();
@@ -237,16 +224,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FP8_THREADS, 1) fp8_
 }
 
 // ------------------------------------------------------------------ host
-// [rows, cols] of a type of esz bytes, boxes of box_rows x box_cols, rows of 128 bytes swizzled
-static bool fp8_map(CUtensorMap* out, CUtensorMapDataType type, int esz, const void* base, uint64_t rows, uint64_t cols, uint32_t box_rows, uint32_t box_cols, bool swizzle) {
-  EncodeTiledFn fn = encode_fn();
-  if (!fn) return false;
-  cuuint64_t dims[2] = {cols, rows}, strides[1] = {cols * esz};
-  cuuint32_t box[2] = {box_cols, box_rows}, estr[2] = {1, 1};
-  return fn(out, type, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
-            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
 typedef void (*Fp8Fn)(Fp8Args);
 struct Fp8Variant { int tn, f32; Fp8Fn fn; int smem; };
 static const Fp8Variant g_fp8[] = {
@@ -277,13 +254,19 @@ static int fp8_ready(int dev) {
 
 using namespace piccl_ops;
 
+constexpr int kFewRows = 64;
+static bool few_takes(const void* x, int fp32, long long stride, int M, long long K) {
+  return M <= kFewRows && !fp32 && K % 8 == 0 && stride % 8 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0;
+}
+
 extern "C" {
 
-// a [M, K], b [N, K], K a multiple of 128, with their scales; out [M, N] bf16 or fp32, rows next to each other; bias [N] bf16 or null.  force_tn: 0, or the tile's width.
+// a [M, K], b [N, K], K a multiple of 128, with their scales; out [M, N] bf16 or fp32, rows next to each other; bias [N] bf16 or null.  force_tn: 0, or the tile's width (for tests).
 int piccl_ops_fp8_gemm(const void* a, const void* sa, const void* b, const void* sb, const void* bias, void* out, int f32, int M, int N, long long K, int force_tn, void* stream) {
   if (M <= 0 || N <= 0 || K <= 0 || K % 128 || K > 0x7fffff00ll || M > 0x7fffff00 || N > 0x7fffff00) return -1;
   for (const void* p : {a, sa, b, sb}) if (!p || (reinterpret_cast<uintptr_t>(p) & 15)) return -2;
   if (!out || (reinterpret_cast<uintptr_t>(out) & (f32 ? 3 : 1)) || (reinterpret_cast<uintptr_t>(bias) & 1)) return -2;
+  if (M <= kFewRows && !force_tn) return fp8_few(nullptr, 0, a, sa, b, sb, bias, out, f32, M, N, (int)K, 0, stream);
   int dev = 0; cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64) return -6;
   const int rc = fp8_ready(dev); if (rc) return rc;
@@ -301,15 +284,33 @@ int piccl_ops_fp8_gemm(const void* a, const void* sa, const void* b, const void*
   g.M = M; g.N = N; g.kb = (int)(K / 128); g.k4 = (g.kb + 3) / 4; g.bias = (const bf16*)bias; g.out = out;
   const int esz = f32 ? 4 : 2;
   g.store_tma = (size_t)N * esz % 16 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0;
-  const auto u8 = CU_TENSOR_MAP_DATA_TYPE_UINT8, u32 = CU_TENSOR_MAP_DATA_TYPE_UINT32;
-  if (!fp8_map(&g.ta, u8, 1, a, M, K, FP8_BM, FP8_BK, true) || !fp8_map(&g.tb, u8, 1, b, N, K, v->tn / 2, FP8_BK, true) ||
-      !fp8_map(&g.sa, u32, 4, sa, (uint64_t)((M + 127) / 128) * g.k4, 128, 1, 128, false) || !fp8_map(&g.sb, u32, 4, sb, (uint64_t)((N + 127) / 128) * g.k4, 128, 1, 128, false)) return -3;
-  if (g.store_tma && !fp8_map(&g.tc, f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, esz, out, M, N, 32, 128 / esz, true)) return -3;
+  if (!fp8_map(&g.ta, 1, a, M, K, FP8_BM, FP8_BK, true) || !fp8_map(&g.tb, 1, b, N, K, v->tn / 2, FP8_BK, true) ||
+      !fp8_map(&g.sa, 4, sa, (uint64_t)((M + 127) / 128) * g.k4, 128, 1, 128, false) || !fp8_map(&g.sb, 4, sb, (uint64_t)((N + 127) / 128) * g.k4, 128, 1, 128, false)) return -3;
+  if (g.store_tma && !fp8_map(&g.tc, esz, out, M, N, 32, 128 / esz, true)) return -3;
   g.status = status_word(STATUS_GEMM);
   if (!g.status) return -7;
   const long tiles = row_tiles * ((N + v->tn - 1) / v->tn);
   const int pairs = (int)(tiles < g_fp8_pairs[dev] ? tiles : g_fp8_pairs[dev]);
   return launch_pdl(v->fn, dim3(2 * pairs), dim3(FP8_THREADS), v->smem, (cudaStream_t)stream, g) == cudaSuccess ? 0 : -5;
+}
+
+
+// out [M, N] = x [M, K] w [N, K]^T + bias, x bf16 (or fp32) with rows `stride` elements apart; keep, keep_s: null, or room for x along its columns in 8 bits ([K, M up to 128]).
+// scratch, scratch_s: room for x in 8 bits, or null where piccl_ops_fp8_linear_scratch says 0.  Returns the number of launches, or a negative code.
+int piccl_ops_fp8_linear_scratch(const void* x, int fp32, long long stride, int M, long long K, int keep) { return keep || !few_takes(x, fp32, stride, M, K); }
+int piccl_ops_fp8_linear(const void* x, int fp32, long long stride, const void* w, const void* sw, const void* bias, void* out, int f32, void* scratch, void* scratch_s, void* keep, void* keep_s, int M,
+                         int N, long long K, void* stream) {
+  if (M <= 0 || N <= 0 || K <= 0 || K > 0x7fffff00ll || stride < K) return -1;
+  if (!piccl_ops_fp8_linear_scratch(x, fp32, stride, M, K, keep != nullptr)) {
+    for (const void* p : {x, w, sw}) if (!p || (reinterpret_cast<uintptr_t>(p) & 15)) return -2;
+    if (!out || (reinterpret_cast<uintptr_t>(out) & (f32 ? 3 : 1)) || (reinterpret_cast<uintptr_t>(bias) & 1)) return -2;
+    const int rc = fp8_few((const bf16*)x, stride, nullptr, nullptr, w, sw, bias, out, f32, M, N, (int)K, 0, stream);
+    return rc ? rc : 1;
+  }
+  if (!scratch || !scratch_s) return -2;
+  int rc = piccl_ops_fp8_quantize(x, fp32, M, K, stride, scratch, scratch_s, keep, keep_s, 0, stream);
+  if (!rc) rc = piccl_ops_fp8_gemm(scratch, scratch_s, w, sw, bias, out, f32, M, N, (K + 127) / 128 * 128, 0, stream);
+  return rc > 0 ? -rc - 100 : rc ? rc : 2;
 }
 
 }  // extern "C"

@@ -11,38 +11,15 @@ struct QuantArgs {
   int c4, r4;                                    // blocks of 512 columns, rows
 };
 
-template <typename T> struct Loads;
-template <> struct Loads<bf16> {
-  static __device__ __forceinline__ void eight(const bf16* p, float (&v)[8]) { unpack8(*reinterpret_cast<const bf16x8*>(p), v); }
-  static __device__ __forceinline__ float one(const bf16* p) { return __bfloat162float(*p); }
-};
-template <> struct Loads<float> {
-  static __device__ __forceinline__ void eight(const float* p, float (&v)[8]) {
-    const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-  }
-  static __device__ __forceinline__ float one(const float* p) { return *p; }
-};
 // columns [c, c + 8) of a row, zeros from C on; VEC: rows start on 16-byte boundaries and C is a multiple of 8
-template <typename T, bool VEC> __device__ __forceinline__ void load8(const T* row, long long c, long long C, float (&v)[8]) {
-  if (VEC) {
-    if (c < C) Loads<T>::eight(row + c, v);
-    else
+template <typename T, bool VEC> __device__ __forceinline__ void load8(const T* row, long long c, long long C, Eight<T>& x) {
 #pragma unroll
-      for (int e = 0; e < 8; e++) v[e] = 0.f;
-  } else {
+  for (int i = 0; i < Eight<T>::W; i++) x.w[i] = 0;
+  if (VEC) { if (c < C) x.load(row + c); }
+  else
 #pragma unroll
-    for (int e = 0; e < 8; e++) v[e] = c + e < C ? Loads<T>::one(row + c + e) : 0.f;
-  }
+    for (int e = 0; e < 8; e++) if (c + e < C) x.set(e, row + c + e);
 }
-__device__ __forceinline__ float scaled(float x, float f) { const float y = x * f; return finite_bits(x) | (x == 0.f) ? y : __uint_as_float(0x7fffffffu); }
-__device__ __forceinline__ uint2 pack_e4m3(const float (&v)[8], float f) {
-  uint2 o;
-  o.x = e4m3_pair(scaled(v[0], f), scaled(v[1], f)) | e4m3_pair(scaled(v[2], f), scaled(v[3], f)) << 16;
-  o.y = e4m3_pair(scaled(v[4], f), scaled(v[5], f)) | e4m3_pair(scaled(v[6], f), scaled(v[7], f)) << 16;
-  return o;
-}
-
 // Along the rows: a warp has a row and 512 columns, a lane 16 of them, so that the four bytes of scales are one word.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) quant_rows_kernel(const QuantArgs a) {
@@ -55,18 +32,18 @@ __global__ void __launch_bounds__(256) quant_rows_kernel(const QuantArgs a) {
   if (row >= a.R) { if (lane == 0) *word = 0x01010101u; return; }
   const T* const x = static_cast<const T*>(a.x) + row * a.stride;
   const long long c = c4 * 512ll + lane * 16;
-  float v[2][8];
+  Eight<T> v[2];
   load8<T, VEC>(x, c, a.C, v[0]);
   load8<T, VEC>(x, c + 8, a.C, v[1]);
-  uint32_t top = 0;
-#pragma unroll
-  for (int e = 0; e < 8; e++) top = max(top, max(finite_bits(v[0][e]), finite_bits(v[1][e])));
+  uint32_t top = max(top8(v[0]), top8(v[1]));
+  const bool odd = __any_sync(0xffffffffu, top >= kInf);
+  if (odd) top = max(finite_top8(v[0]), finite_top8(v[1]));
 #pragma unroll
   for (int o = 4; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
   const uint32_t byte = scale_byte(top);
   const float f = scale_inverse(byte);
   if (c < a.kc) {
-    const uint2 lo = pack_e4m3(v[0], f), hi = pack_e4m3(v[1], f);
+    const uint2 lo = pack_row(v[0], f, odd), hi = pack_row(v[1], f, odd);
     *reinterpret_cast<uint4*>(a.q + row * a.kc + c) = make_uint4(lo.x, lo.y, hi.x, hi.y);
   }
   uint32_t all = byte << (8 * (lane >> 3));
@@ -75,33 +52,44 @@ __global__ void __launch_bounds__(256) quant_rows_kernel(const QuantArgs a) {
   if (lane == 0) *word = all;
 }
 
-// A block has a tile of 128 x 128 in registers, a thread 8 x 8 of it (16 lanes beside each other to a row).
+// A block has a tile of 128 x 128 in registers as it came, a thread 8 x 8 of it (16 lanes beside each other to a row).
 template <typename T, bool VEC, bool ROWS, bool COLS, bool SQUARE>
-__global__ void __launch_bounds__(256) quant_tile_kernel(const QuantArgs a) {
-  __shared__ uint32_t tops[16][128];
-  __shared__ __align__(16) uint8_t turned[128 * 128];
-  __shared__ uint8_t bytes[128];
+__global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2) quant_tile_kernel(const QuantArgs a) {
+  constexpr int W = Eight<T>::W;
+  __shared__ __align__(16) uint8_t turned[COLS ? 128 * 128 : 16];
+  __shared__ __align__(16) uint32_t tops[SQUARE || !COLS ? 1 : 16][SQUARE || !COLS ? 8 : 16 * W];
+  __shared__ __align__(8) uint8_t bytes[128];
   pdl_begin();
   const int cg = threadIdx.x & 15, rg = threadIdx.x >> 4;
-  const long long r0 = blockIdx.y * 128ll + rg * 8, c0 = blockIdx.x * 128ll + cg * 8;
-  float v[8][8];
+  const int bx = blockIdx.x % (int)(a.kc >> 7), by = blockIdx.x / (int)(a.kc >> 7);
+  const long long r0 = by * 128ll + rg * 8, c0 = bx * 128ll + cg * 8;
+  Eight<T> v[8];
 #pragma unroll
   for (int i = 0; i < 8; i++) {
     if (r0 + i < a.R) load8<T, VEC>(static_cast<const T*>(a.x) + (r0 + i) * a.stride, c0, a.C, v[i]);
     else
 #pragma unroll
-      for (int e = 0; e < 8; e++) v[i][e] = 0.f;
+      for (int e = 0; e < W; e++) v[i].w[e] = 0;
   }
-  const int bx = blockIdx.x, by = blockIdx.y;
+  // the largest magnitudes of the thread's columns, and of all
+  uint32_t col[W], top = 0;
+#pragma unroll
+  for (int e = 0; e < W; e++) {
+    col[e] = Eight<T>::magnitude(v[0].w[e]);
+#pragma unroll
+    for (int i = 1; i < 8; i++) col[e] = Eight<T>::most(col[e], Eight<T>::magnitude(v[i].w[e]));
+    top = max(top, sizeof(T) == 2 ? max(col[e] & 0xffff0000u, col[e] << 16) : col[e]);
+  }
+  const bool odd = __syncthreads_or(top >= kInf);
   // bytes of blocks beyond the last one, up to a whole word
-  const int more_c = bx + 1 == (int)gridDim.x ? 4 * a.c4 - bx : 1, more_r = by + 1 == (int)gridDim.y ? 4 * a.r4 - by : 1;
+  const int more_c = bx + 1 == (int)(a.kc >> 7) ? 4 * a.c4 - bx : 1, more_r = by + 1 == (int)(a.kr >> 7) ? 4 * a.r4 - by : 1;
   float square = 0.f;
   if (SQUARE) {
-    uint32_t top = 0;
+    if (odd) {
+      top = 0;
 #pragma unroll
-    for (int i = 0; i < 8; i++)
-#pragma unroll
-      for (int e = 0; e < 8; e++) top = max(top, finite_bits(v[i][e]));
+      for (int i = 0; i < 8; i++) top = max(top, finite_top8(v[i]));
+    }
     top = __reduce_max_sync(0xffffffffu, top);
     if ((threadIdx.x & 31) == 0) tops[0][threadIdx.x >> 5] = top;
     __syncthreads();
@@ -119,53 +107,62 @@ __global__ void __launch_bounds__(256) quant_tile_kernel(const QuantArgs a) {
     for (int i = 0; i < 8; i++) {
       float f = square;
       if (!SQUARE) {
-        uint32_t top = 0;
+        uint32_t t = odd ? finite_top8(v[i]) : top8(v[i]);
 #pragma unroll
-        for (int e = 0; e < 8; e++) top = max(top, finite_bits(v[i][e]));
-#pragma unroll
-        for (int o = 8; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-        const uint32_t byte = scale_byte(top);
+        for (int o = 8; o > 0; o >>= 1) t = max(t, __shfl_xor_sync(0xffffffffu, t, o));
+        const uint32_t byte = scale_byte(t);
         f = scale_inverse(byte);
         if (cg == 0) for (int k = 0; k < more_c; k++) a.qs[scale_at(r0 + i, bx + k, a.c4)] = k ? 1 : byte;
       }
-      if (r0 + i < a.R) *reinterpret_cast<uint2*>(a.q + (r0 + i) * a.kc + c0) = pack_e4m3(v[i], f);
+      if (r0 + i < a.R) *reinterpret_cast<uint2*>(a.q + (r0 + i) * a.kc + c0) = pack_row(v[i], f, odd);
     }
   }
   if (COLS) {
     if (!SQUARE) {
+      if (odd) {
 #pragma unroll
-      for (int e = 0; e < 8; e++) {
-        uint32_t top = 0;
+        for (int e = 0; e < W; e++) {
+          uint32_t m[2] = {0, 0};
 #pragma unroll
-        for (int i = 0; i < 8; i++) top = max(top, finite_bits(v[i][e]));
-        tops[rg][cg * 8 + e] = top;
+          for (int i = 0; i < 8; i++)
+#pragma unroll
+            for (int h = 0; h < 8 / W; h++) m[h] = max(m[h], finite_bits(v[i].at(8 / W * e + h)));
+          col[e] = sizeof(T) == 2 ? m[0] >> 16 | (m[1] & 0xffff0000u) : m[0];
+        }
       }
-      __syncthreads();
-      if (threadIdx.x < 128) {
-        uint32_t top = 0;
 #pragma unroll
-        for (int g = 0; g < 16; g++) top = max(top, tops[g][threadIdx.x]);
-        const uint32_t byte = scale_byte(top);
-        bytes[threadIdx.x] = byte;
-        for (int k = 0; k < more_r; k++) a.ts[scale_at(bx * 128ll + threadIdx.x, by + k, a.r4)] = k ? 1 : byte;
+      for (int e = 0; e < W; e += 4) *reinterpret_cast<uint4*>(&tops[rg][cg * W + e]) = make_uint4(col[e], col[e + 1], col[e + 2], col[e + 3]);
+      __syncthreads();
+      if (threadIdx.x < 16 * W) {
+        uint32_t m = tops[0][threadIdx.x];
+#pragma unroll
+        for (int g = 1; g < 16; g++) m = Eight<T>::most(m, tops[g][threadIdx.x]);
+#pragma unroll
+        for (int h = 0; h < 8 / W; h++) {
+          const int c = threadIdx.x * (8 / W) + h;
+          const uint32_t byte = scale_byte(Eight<T>::bits(m, h));
+          bytes[c] = byte;
+          for (int k = 0; k < more_r; k++) a.ts[scale_at(bx * 128ll + c, by + k, a.r4)] = k ? 1 : byte;
+        }
       }
       __syncthreads();
     }
     // eight rows of a column are 8 bytes of the turned tile; their place in its row of 16 is moved by the column, or 16 lanes would meet in one bank
+    const uint2 eight = SQUARE ? make_uint2(0, 0) : *reinterpret_cast<const uint2*>(bytes + cg * 8);
 #pragma unroll
     for (int e = 0; e < 8; e++) {
+      const float f = SQUARE ? square : scale_inverse(((e < 4 ? eight.x : eight.y) >> (8 * (e & 3))) & 255u);
       float w[8];
 #pragma unroll
-      for (int i = 0; i < 8; i++) w[i] = v[i][e];
-      const float f = SQUARE ? square : scale_inverse(bytes[cg * 8 + e]);
-      *reinterpret_cast<uint2*>(turned + (cg * 8 + e) * 128 + ((rg ^ cg) << 3)) = pack_e4m3(w, f);
+      for (int i = 0; i < 8; i++) { w[i] = v[i].at(e); if (odd) w[i] = nan_of_inf(w[i]); }
+      *reinterpret_cast<uint2*>(turned + (cg * 8 + e) * 128 + ((rg ^ cg) << 3)) = make_uint2(pack4(w[0], w[1], w[2], w[3], f), pack4(w[4], w[5], w[6], w[7], f));
     }
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < 8; i++) {
-      const int col = i * 16 + rg;
-      if (bx * 128ll + col < a.C)
-        *reinterpret_cast<uint2*>(a.t + (bx * 128ll + col) * a.kr + by * 128ll + cg * 8) = *reinterpret_cast<const uint2*>(turned + col * 128 + ((cg ^ (col >> 3)) << 3));
+      const int c = i * 16 + rg;
+      if (bx * 128ll + c < a.C)
+        *reinterpret_cast<uint2*>(a.t + (bx * 128ll + c) * a.kr + by * 128ll + cg * 8) = *reinterpret_cast<const uint2*>(turned + c * 128 + ((cg ^ (c >> 3)) << 3));
     }
   }
 }
@@ -176,7 +173,7 @@ static cudaError_t quantize(const QuantArgs& a, int square, cudaStream_t s) {
     const long long warps = (a.R + 127) / 128 * 128 * a.c4;
     return launch_pdl(quant_rows_kernel<T, VEC>, dim3((unsigned)((warps + 7) / 8)), 256, 0, s, a);
   }
-  const dim3 grid((unsigned)(a.kc / 128), (unsigned)(a.kr / 128));
+  const dim3 grid((unsigned)(a.kc / 128 * (a.kr / 128)));
   if (square) return launch_pdl(a.t ? (a.q ? quant_tile_kernel<T, VEC, true, true, true> : quant_tile_kernel<T, VEC, false, true, true>) : quant_tile_kernel<T, VEC, true, false, true>, grid, 256, 0, s, a);
   return launch_pdl(a.q ? quant_tile_kernel<T, VEC, true, true, false> : quant_tile_kernel<T, VEC, false, true, false>, grid, 256, 0, s, a);
 }
@@ -195,8 +192,7 @@ int piccl_ops_fp8_quantize(const void* x, int fp32, long long R, long long C, lo
   const uintptr_t esz = fp32 ? 4 : 2;
   if ((reinterpret_cast<uintptr_t>(x) & (esz - 1)) || ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(t) | reinterpret_cast<uintptr_t>(qs) | reinterpret_cast<uintptr_t>(ts)) & 15)) return -2;
   QuantArgs a{x, stride, (uint8_t*)q, (uint8_t*)qs, (uint8_t*)t, (uint8_t*)ts, R, C, (C + 127) / 128 * 128, (R + 127) / 128 * 128, (int)((C + 511) / 512), (int)((R + 511) / 512)};
-  if (a.kr / 128 > 65535 && (t || square)) return -1;                     // rows of tiles of a grid
-  if (a.kr * a.c4 / 8 > 0x7fffffffll) return -1;
+  if ((a.kr / 128) * (a.kc / 128) > 0x7fffffffll || a.kr * a.c4 / 8 > 0x7ffffff0ll) return -1;      // blocks of a grid
   const bool vec = C % 8 == 0 && stride * esz % 16 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0;
   const cudaStream_t s = (cudaStream_t)stream;
   const cudaError_t e = fp32 ? (vec ? quantize<float, true>(a, square, s) : quantize<float, false>(a, square, s)) : (vec ? quantize<bf16, true>(a, square, s) : quantize<bf16, false>(a, square, s));

@@ -87,3 +87,31 @@ def test_product(M, N, K, tile, dtype):
     ops.raise_if_a_wait_ran_out()
     assert bool((off <= bound).all())
     assert torch.isnan(guard[M]).all()
+
+
+@pytest.mark.parametrize("M", [1, 2, 15, 16, 17, 31, 33, 64, 65])
+@pytest.mark.parametrize("N,K", [(1, 8), (128, 128), (257, 640), (1000, 1096), (4096, 1024), (520, 4104), (136, 72), (64, 333)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_linear_of_few_rows(M, N, K, dtype):
+    """One launch up to 64 rows where they lie on 16-byte boundaries: the same bits as the quantiser and a product in 64 bits, within that product's bound."""
+    from piccl_b200 import ops
+    from piccl_b200.ops import fp8
+    x = _randn(M, K, seed=M) * torch.exp(_randn(M, 1, seed=2) * 2)
+    w, q = fp8.empty(N, K), fp8.empty(M, K)
+    fp8.quantize(_randn(N, K, seed=3, scale=0.02), w, square=True)
+    fp8.quantize(x, q)
+    bias = _randn(N, seed=4) if M % 2 else None
+    a, b = fp8.dequantize(q).double(), fp8.dequantize(w).double()
+    want, size = a @ b.t(), a.abs() @ b.t().abs()
+    if bias is not None:
+        want, size = want + bias.double(), size + bias.double().abs()
+    bound = 2 * EPS32 * (K / 32 + 2 + 8) * size + (EPS16 if dtype == torch.bfloat16 else EPS32) * want.abs()          # sums of up to 8 slices
+    for call in ("linear", "product"):
+        guard = torch.full((M + 1, N), math.nan, device="cuda", dtype=dtype)
+        if call == "linear":
+            fp8.linear(x, w, guard[:M], bias=bias)
+        else:
+            fp8.product(q, w, guard[:M], bias=bias)
+        ops.raise_if_a_wait_ran_out()
+        assert bool(((guard[:M].double() - want).abs() <= bound).all()), call
+        assert torch.isnan(guard[M]).all()
