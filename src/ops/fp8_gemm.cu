@@ -19,7 +19,7 @@ struct Fp8Args {
   CUtensorMap ta, tb, sa, sb, tc;
   const bf16* bias;
   void* out;
-  int M, N, kb, k4, store_tma;       // k-blocks of 128, words of four of them
+  int M, N, kb, k4, store_tma, bias_words;       // k-blocks of 128, words of four of them
   int* status;
 };
 
@@ -36,7 +36,8 @@ struct Fp8Smem {
   static_assert(DYNAMIC <= 232448, "more shared memory than a CTA can have");
 };
 
-template <typename O> struct OutPiece;                     // 128 bytes of a row
+// 128 bytes of a row of the result
+template <typename O> struct OutPiece;
 template <> struct OutPiece<bf16> {
   static constexpr int COLS = 64;
   static __device__ __forceinline__ void stage(uint8_t* row, int r, const float (&v)[64]) {
@@ -56,11 +57,43 @@ template <> struct OutPiece<float> {
     for (int j = 0; j < 8; j++) *reinterpret_cast<float4*>(row + ((j ^ (r & 7)) << 4)) = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
   }
 };
+// Rows of a result that do not start on 16 bytes, which no TMA store takes: a warp writes a row at a time, a word of 4 bytes a lane.  Rows of bf16 that begin in the middle of a word are
+// moved by half a word, their first and last value written on their own.  left: columns that are there.
+__device__ __forceinline__ void store_rows(const uint8_t* staging, float* out, size_t stride, int rows, int left, int lane) {
+#pragma unroll 8
+  for (int r = 0; r < 32; r++) {
+    const float v = *reinterpret_cast<const float*>(staging + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4);
+    if (r < rows && lane < left) out[r * stride + lane] = v;
+  }
+}
+__device__ __forceinline__ void store_rows(const uint8_t* staging, bf16* out, size_t stride, int rows, int left, int lane) {
+#pragma unroll 8
+  for (int r = 0; r < 32; r++) {
+    const uint32_t w = *reinterpret_cast<const uint32_t*>(staging + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4), next = __shfl_down_sync(0xffffffffu, w, 1);
+    uint16_t* const o = reinterpret_cast<uint16_t*>(out + r * stride);
+    if (r >= rows) continue;
+    if ((reinterpret_cast<uintptr_t>(o) & 2) == 0) {
+      if (2 * lane + 1 < left) reinterpret_cast<uint32_t*>(o)[lane] = w;
+      else if (2 * lane < left) o[2 * lane] = (uint16_t)w;
+    } else {
+      if (lane == 0) o[0] = (uint16_t)w;
+      if (2 * lane + 2 < left && lane < 31) *reinterpret_cast<uint32_t*>(o + 2 * lane + 1) = __funnelshift_r(w, next, 16);
+      else if (2 * lane + 1 < left) o[2 * lane + 1] = (uint16_t)(w >> 16);
+    }
+  }
+}
 
+// A tile's sum is one unit, or several that the epilogue adds up: the tensor core cuts its fp32 sums off where an fma would round them, always toward zero, which over K / 32 steps loses
+// 2^-25 K / 48 of a sum of random signs (measured 1.6e-6 at K = 2331).  That is nothing to a result in bf16; one in fp32 is added up from units of 1024 k, rounded, in registers.
+constexpr int kUnit = 8;           // k-blocks (tiles of 128 columns at most: 64 sums a thread; 128 do not fit beside the rest into the 168 registers that ten warps can have)
+
+// TMEM has 512 columns: two accumulators of 256 and the scales do not fit.  They overlap in 16 columns: the MMAs of the next unit wait until the epilogue has those in registers (its warps
+// take the piece with them first), and not for the rest of the tile.
 template <int TN, int STAGES, typename O>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FP8_THREADS, 1) fp8_pair_kernel(const __grid_constant__ Fp8Args a) {
   typedef Fp8Smem<TN, STAGES> L;
-  constexpr int ACCS = TN <= 128 ? 2 : 1;
+  constexpr bool OVERLAP = TN > 240, ADD = sizeof(O) == 4;
+  constexpr uint32_t ACC = OVERLAP ? 240 : TN;            // columns between the accumulators
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   __shared__ int s_abort;
   uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -69,6 +102,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FP8_THREADS, 1) fp8_
   uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(tmem_empty + 2);
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31, v = (int)cluster_ctarank();
   const int num_m = (a.M + 255) / 256, num_n = (a.N + TN - 1) / TN, num_tiles = num_m * num_n, first = blockIdx.x >> 1, stride = gridDim.x >> 1;
+  const int units = ADD ? (a.kb + kUnit - 1) / kUnit : 1;
   auto tile = [&](int t, int& m_blk, int& n_blk) {         // bands of 16 row tiles, as in gemm_sm100.cu
     const int per_band = 16 * num_n, band = t / per_band, within = t % per_band, rows = min(16, num_m - band * 16);
     m_blk = 2 * (band * 16 + within % rows) + v; n_blk = within / rows;
@@ -120,92 +154,146 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FP8_THREADS, 1) fp8_
       const uint64_t da0 = make_smem_desc_k128(smem), db0 = make_smem_desc_k128(smem + L::A_BYTES), ds0 = make_smem_desc_scales(smem + L::SF_OFF);
       const uint32_t sfa = tmem + kScaleCol, sfb = sfa + 4;
       int stage = 0; uint32_t phase = 0; int local = 0;
-      for (int t = first; t < num_tiles && !*(volatile int*)&s_abort; t += stride, local++) {
+      bool ok = true;
+      for (int t = first; ok && t < num_tiles && !*(volatile int*)&s_abort; t += stride) {
         int m_blk, n_blk; tile(t, m_blk, n_blk);
-        const int acc = local % ACCS; const uint32_t acc_phase = (local / ACCS) & 1;
-        if (!mbar_wait(&tmem_empty[acc], acc_phase ^ 1, &s_abort, kPairWaitLimitNs)) { if (issuer) atomicExch(a.status, 12); break; }
-        tc_fence_after();
-        const uint32_t d = tmem + acc * TN;
         const uint32_t sfb_t = sfb + (TN == 64 ? 2 * (n_blk & 1) : 0);
-        bool ok = true;
-        for (int kb = 0; kb < a.kb; kb++) {
-          if (!mbar_wait(&full[stage], phase, &s_abort, kPairWaitLimitNs)) { if (issuer) atomicExch(a.status, 13); ok = false; break; }
-          tc_fence_after();
-          const uint64_t da = desc_advance(da0, stage * L::STAGE), db = desc_advance(db0, stage * L::STAGE);
-          if (issuer) {
-            if ((kb & 3) == 0) {
-              const uint64_t ds = desc_advance(ds0, stage * L::SF_BYTES);
-              scales_to_tmem_pair(sfa, ds);
-              scales_to_tmem_pair(sfb, desc_advance(ds, 512));
-              if (TN > 128) scales_to_tmem_pair(sfb + 4, desc_advance(ds, 1024));
-            }
-#pragma unroll
-            for (int k = 0; k < FP8_BK / 32; k++) umma_mxf8_pair(d, desc_advance(da, k * 32), desc_advance(db, k * 32), idesc | idesc_bytes(kb & 3, kb & 3), sfa, sfb_t, kb != 0 || k != 0);
-            umma_commit_pair(&empty[stage]);
+        for (int u = 0; ok && u < units; u++, local++) {
+          const int acc = local & 1;
+          // overlapping: the edge of the unit before is in registers, and with it all of the one before that; else: this accumulator's unit is
+          if (OVERLAP ? local > 0 && !mbar_wait(&tmem_empty[0], (local - 1) & 1, &s_abort, kPairWaitLimitNs) : !mbar_wait(&tmem_empty[acc], ((local >> 1) & 1) ^ 1, &s_abort, kPairWaitLimitNs)) {
+            if (issuer) atomicExch(a.status, 12);
+            ok = false; break;
           }
+          tc_fence_after();
+          const uint32_t d = tmem + acc * ACC;
+          const int kb0 = ADD ? u * kUnit : 0, kb1 = ADD ? min(a.kb, kb0 + kUnit) : a.kb;
+          for (int kb = kb0; kb < kb1; kb++) {
+            if (!mbar_wait(&full[stage], phase, &s_abort, kPairWaitLimitNs)) { if (issuer) atomicExch(a.status, 13); ok = false; break; }
+            tc_fence_after();
+            const uint64_t da = desc_advance(da0, stage * L::STAGE), db = desc_advance(db0, stage * L::STAGE);
+            if (issuer) {
+              if ((kb & 3) == 0) {
+                const uint64_t ds = desc_advance(ds0, stage * L::SF_BYTES);
+                scales_to_tmem_pair(sfa, ds);
+                scales_to_tmem_pair(sfb, desc_advance(ds, 512));
+                if (TN > 128) scales_to_tmem_pair(sfb + 4, desc_advance(ds, 1024));
+              }
+#pragma unroll
+              for (int k = 0; k < FP8_BK / 32; k++) umma_mxf8_pair(d, desc_advance(da, k * 32), desc_advance(db, k * 32), idesc | idesc_bytes(kb & 3, kb & 3), sfa, sfb_t, kb != kb0 || k != 0);
+              umma_commit_pair(&empty[stage]);
+            }
+            __syncwarp();
+            if (++stage == STAGES) { stage = 0; phase ^= 1; }
+          }
+          if (ok && issuer) umma_commit_pair(&tmem_full[acc]);
           __syncwarp();
-          if (++stage == STAGES) { stage = 0; phase ^= 1; }
         }
-        if (!ok) break;
-        if (issuer) umma_commit_pair(&tmem_full[acc]);
-        __syncwarp();
       }
     }
   } else {
     typedef OutPiece<O> P;
     constexpr int PIECES = TN / P::COLS, PER = PIECES >= 2 ? PIECES / 2 : 1;
-    EpiCtx e;
-    e.quarter = warp & 3; e.half = (warp - 2) >> 2; e.lane = lane;
-    e.staging = smem + L::STAGING_OFF + (warp - 2) * PAIR_STAGING;
+    const int quarter = warp & 3, half = (warp - 2) >> 2;
+    uint8_t* const staging = smem + L::STAGING_OFF + (warp - 2) * PAIR_STAGING;
+    const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
     int local = 0;
-    for (int t = first; t < num_tiles; t += stride, local++) {
+    bool ok = true;
+    for (int t = first; ok && t < num_tiles; t += stride) {
       int m_blk, n_blk; tile(t, m_blk, n_blk);
-      const int acc = local % ACCS; const uint32_t acc_phase = (local / ACCS) & 1;
-      e.tmem = tmem + ((uint32_t)(e.quarter * 32) << 16) + acc * TN;
-      if (!mbar_wait(&tmem_full[acc], acc_phase, &s_abort, kPairWaitLimitNs)) { atomicExch(a.status, 14); break; }
-      tc_fence_after();
-      const int row0 = m_blk * FP8_BM + e.quarter * 32;
-      if (row0 < a.M && (PIECES >= 2 || e.half == 0)) {
-#pragma unroll 1
-        for (int pc = e.half * PER; pc < e.half * PER + PER; pc++) {
-          const int col = n_blk * TN + pc * P::COLS;
-          if (col >= a.N) break;
-          float x[P::COLS];
+      const int row0 = m_blk * FP8_BM + quarter * 32;
+      const bool mine = row0 < a.M && (PIECES >= 2 || half == 0);
+      // a piece of the thread's row on its way out
+      auto ship = [&](float (&x)[P::COLS], int pc) {
+        const int col = n_blk * TN + pc * P::COLS;
+        if (col >= a.N) return;
+        if (a.bias) {
+          if (col + P::COLS <= a.N && a.bias_words) {
 #pragma unroll
-          for (int q = 0; q < P::COLS / 32; q++) {
-            uint32_t r[32];
-            tmem_ld_32x32(e.tmem + pc * P::COLS + 32 * q, r);
-            tmem_ld_wait();
+            for (int j = 0; j < P::COLS; j += 8) {
+              float f[8]; unpack8(*reinterpret_cast<const bf16x8*>(a.bias + col + j), f);
 #pragma unroll
-            for (int i = 0; i < 32; i++) x[32 * q + i] = __uint_as_float(r[i]);
-          }
-          if (a.bias) {
+              for (int q = 0; q < 8; q++) x[j + q] += f[q];
+            }
+          } else {
 #pragma unroll
-            for (int i = 0; i < P::COLS; i++) x[i] += __bfloat162float(a.bias[min(col + i, a.N - 1)]);
-          }
-          epi_staging_free(e);
-          P::stage(e.staging + lane * 128, lane, x);
-          if (a.store_tma) {
-            fence_proxy_async();
-            __syncwarp();
-            epi_ship(e, &a.tc, col, row0);
-          } else {                                         // rows that do not start on 16 bytes: a row at a time
-            __syncwarp();
-            O* const out = static_cast<O*>(a.out);
-            for (int r = 0; r < 32 && row0 + r < a.M; r++)
-#pragma unroll
-              for (int c = lane; c < P::COLS; c += 32)
-                if (col + c < a.N) {
-                  const int byte = c * (int)sizeof(O);
-                  out[(size_t)(row0 + r) * a.N + col + c] = *reinterpret_cast<const O*>(e.staging + r * 128 + (((byte >> 4) ^ (r & 7)) << 4) + (byte & 15));
-                }
-            __syncwarp();
+            for (int j = 0; j < P::COLS; j++) x[j] += __bfloat162float(a.bias[min(col + j, a.N - 1)]);
           }
         }
+        if (lane == 0) bulk_wait_read_all();               // the last store has been read out of the staging buffer
+        __syncwarp();
+        P::stage(staging + lane * 128, lane, x);
+        if (a.store_tma) {
+          fence_proxy_async();
+          __syncwarp();
+          if (lane == 0) { tma_store_2d(&a.tc, staging, col, row0); bulk_commit(); }
+        } else {
+          __syncwarp();
+          store_rows(staging, static_cast<O*>(a.out) + (size_t)row0 * a.N + col, a.N, a.M - row0, a.N - col, lane);
+          __syncwarp();
+        }
+      };
+      // waits for a unit; true: this warp's columns are among those that the accumulators share, and it reports when it has them
+      auto arrived = [&](bool& edge) {
+        edge = OVERLAP && half == ((local & 1) ^ 1) && mine;
+        if (!mbar_wait(&tmem_full[local & 1], (local >> 1) & 1, &s_abort, kPairWaitLimitNs)) { atomicExch(a.status, 14); return false; }
+        tc_fence_after();
+        if (OVERLAP && !edge && lane == 0) mbar_arrive_leader(&tmem_empty[0]);
+        return true;
+      };
+      auto taken = [&](uint64_t* bar) { tc_fence_before(); __syncwarp(); if (lane == 0) mbar_arrive_leader(bar); };
+      bool edge;
+      if constexpr (ADD) {
+        float sum[PER][P::COLS];
+#pragma unroll
+        for (int i = 0; i < PER; i++)
+#pragma unroll
+          for (int j = 0; j < P::COLS; j++) sum[i][j] = 0.f;
+#pragma unroll 1
+        for (int u = 0; u < units; u++, local++) {
+          if (!arrived(edge)) { ok = false; break; }
+          if (mine) {
+#pragma unroll
+            for (int i = 0; i < PER; i++) {
+#pragma unroll
+              for (int q = 0; q < P::COLS / 16; q++) {     // few columns at a time: the sums leave few registers
+                uint32_t r[16];
+                tmem_ld_32x16(lanes + (local & 1) * ACC + (half ? PIECES - 1 - i : i) * P::COLS + 16 * q, r);
+                tmem_ld_wait();
+#pragma unroll
+                for (int j = 0; j < 16; j++) sum[i][16 * q + j] += __uint_as_float(r[j]);
+              }
+              if (i == 0 && edge) taken(&tmem_empty[0]);
+            }
+          }
+          if (!OVERLAP) taken(&tmem_empty[local & 1]);
+        }
+        if (ok && mine) {
+#pragma unroll
+          for (int i = 0; i < PER; i++) ship(sum[i], half ? PIECES - 1 - i : i);
+        }
+      } else {
+        if (!arrived(edge)) { ok = false; break; }
+        if (mine) {
+#pragma unroll 1
+          for (int i = 0; i < PER; i++) {
+            const int pc = half ? PIECES - 1 - i : i;
+            float x[P::COLS];
+#pragma unroll
+            for (int q = 0; q < P::COLS / 32; q++) {
+              uint32_t r[32];
+              tmem_ld_32x32(lanes + (local & 1) * ACC + pc * P::COLS + 32 * q, r);
+              tmem_ld_wait();
+#pragma unroll
+              for (int j = 0; j < 32; j++) x[32 * q + j] = __uint_as_float(r[j]);
+            }
+            if (i == 0 && edge) taken(&tmem_empty[0]);
+            ship(x, pc);
+          }
+        }
+        if (!OVERLAP) taken(&tmem_empty[local & 1]);
+        local++;
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive_leader(&tmem_empty[acc]);
     }
   }
   // the ending of gemm_pair_persistent: nobody leaves while the other CTA may still touch its shared memory or barriers
@@ -228,7 +316,7 @@ typedef void (*Fp8Fn)(Fp8Args);
 struct Fp8Variant { int tn, f32; Fp8Fn fn; int smem; };
 static const Fp8Variant g_fp8[] = {
   {256, 0, fp8_pair_kernel<256, 5, bf16>, Fp8Smem<256, 5>::DYNAMIC}, {128, 0, fp8_pair_kernel<128, 7, bf16>, Fp8Smem<128, 7>::DYNAMIC}, {64, 0, fp8_pair_kernel<64, 8, bf16>, Fp8Smem<64, 8>::DYNAMIC},
-  {256, 1, fp8_pair_kernel<256, 5, float>, Fp8Smem<256, 5>::DYNAMIC}, {128, 1, fp8_pair_kernel<128, 7, float>, Fp8Smem<128, 7>::DYNAMIC}, {64, 1, fp8_pair_kernel<64, 8, float>, Fp8Smem<64, 8>::DYNAMIC},
+  {128, 1, fp8_pair_kernel<128, 7, float>, Fp8Smem<128, 7>::DYNAMIC}, {64, 1, fp8_pair_kernel<64, 8, float>, Fp8Smem<64, 8>::DYNAMIC},
 };
 static int g_fp8_pairs[64] = {0};
 
@@ -287,6 +375,7 @@ int piccl_ops_fp8_gemm(const void* a, const void* sa, const void* b, const void*
   if (!fp8_map(&g.ta, 1, a, M, K, FP8_BM, FP8_BK, true) || !fp8_map(&g.tb, 1, b, N, K, v->tn / 2, FP8_BK, true) ||
       !fp8_map(&g.sa, 4, sa, (uint64_t)((M + 127) / 128) * g.k4, 128, 1, 128, false) || !fp8_map(&g.sb, 4, sb, (uint64_t)((N + 127) / 128) * g.k4, 128, 1, 128, false)) return -3;
   if (g.store_tma && !fp8_map(&g.tc, esz, out, M, N, 32, 128 / esz, true)) return -3;
+  g.bias_words = reinterpret_cast<uintptr_t>(bias) % 16 == 0;
   g.status = status_word(STATUS_GEMM);
   if (!g.status) return -7;
   const long tiles = row_tiles * ((N + v->tn - 1) / v->tn);
