@@ -57,28 +57,39 @@ template <> struct OutPiece<float> {
     for (int j = 0; j < 8; j++) *reinterpret_cast<float4*>(row + ((j ^ (r & 7)) << 4)) = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
   }
 };
-// Rows of a result that do not start on 16 bytes, which no TMA store takes: a warp writes a row at a time, a word of 4 bytes a lane.  Rows of bf16 that begin in the middle of a word are
-// moved by half a word, their first and last value written on their own.  left: columns that are there.
+// Rows of a result that do not start on 16 bytes, which no TMA store takes: a warp writes a row at a time, a word of 4 bytes a lane, from words of 16 rows that it has loaded (row by row, each
+// waiting for its load, a row took 200 clocks).  Rows of bf16 that begin in the middle of a word are moved by half a word, their first and last value written on their own.
+// left: columns that are there.
+__device__ __forceinline__ uint32_t staged_word(const uint8_t* staging, int r, int lane) {
+  return *reinterpret_cast<const uint32_t*>(staging + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4);
+}
 __device__ __forceinline__ void store_rows(const uint8_t* staging, float* out, size_t stride, int rows, int left, int lane) {
-#pragma unroll 8
-  for (int r = 0; r < 32; r++) {
-    const float v = *reinterpret_cast<const float*>(staging + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4);
-    if (r < rows && lane < left) out[r * stride + lane] = v;
+#pragma unroll
+  for (int r0 = 0; r0 < 32; r0 += 16) {
+    uint32_t w[16];
+#pragma unroll
+    for (int r = 0; r < 16; r++) w[r] = staged_word(staging, r0 + r, lane);
+#pragma unroll
+    for (int r = 0; r < 16; r++) if (r0 + r < rows && lane < left) out[(r0 + r) * stride + lane] = __uint_as_float(w[r]);
   }
 }
 __device__ __forceinline__ void store_rows(const uint8_t* staging, bf16* out, size_t stride, int rows, int left, int lane) {
-#pragma unroll 8
-  for (int r = 0; r < 32; r++) {
-    const uint32_t w = *reinterpret_cast<const uint32_t*>(staging + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4), next = __shfl_down_sync(0xffffffffu, w, 1);
-    uint16_t* const o = reinterpret_cast<uint16_t*>(out + r * stride);
-    if (r >= rows) continue;
-    if ((reinterpret_cast<uintptr_t>(o) & 2) == 0) {
-      if (2 * lane + 1 < left) reinterpret_cast<uint32_t*>(o)[lane] = w;
-      else if (2 * lane < left) o[2 * lane] = (uint16_t)w;
-    } else {
-      if (lane == 0) o[0] = (uint16_t)w;
-      if (2 * lane + 2 < left && lane < 31) *reinterpret_cast<uint32_t*>(o + 2 * lane + 1) = __funnelshift_r(w, next, 16);
-      else if (2 * lane + 1 < left) o[2 * lane + 1] = (uint16_t)(w >> 16);
+#pragma unroll
+  for (int r0 = 0; r0 < 32; r0 += 16) {
+    uint32_t w[16], n[16];
+#pragma unroll
+    for (int r = 0; r < 16; r++) w[r] = staged_word(staging, r0 + r, lane);
+#pragma unroll
+    for (int r = 0; r < 16; r++) n[r] = __shfl_down_sync(0xffffffffu, w[r], 1);
+#pragma unroll
+    for (int r = 0; r < 16; r++) {
+      uint16_t* const o = reinterpret_cast<uint16_t*>(out + (r0 + r) * stride);
+      const int odd = (int)(reinterpret_cast<uintptr_t>(o) >> 1) & 1, c = 2 * lane + odd;
+      const uint32_t x = odd ? __funnelshift_r(w[r], n[r], 16) : w[r];
+      const bool there = r0 + r < rows, whole = c + 1 < left && c < 63;
+      if (there && whole) *reinterpret_cast<uint32_t*>(o + c) = x;
+      if (there && !whole && c < left) o[c] = (uint16_t)x;
+      if (there && odd && lane == 0) o[0] = (uint16_t)w[r];
     }
   }
 }
@@ -93,6 +104,7 @@ template <int TN, int STAGES, typename O>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FP8_THREADS, 1) fp8_pair_kernel(const __grid_constant__ Fp8Args a) {
   typedef Fp8Smem<TN, STAGES> L;
   constexpr bool OVERLAP = TN > 240, ADD = sizeof(O) == 4;
+  static_assert(!(OVERLAP && ADD), "128 sums a thread do not fit");
   constexpr uint32_t ACC = OVERLAP ? 240 : TN;            // columns between the accumulators
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   __shared__ int s_abort;
@@ -244,33 +256,31 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FP8_THREADS, 1) fp8_
       auto taken = [&](uint64_t* bar) { tc_fence_before(); __syncwarp(); if (lane == 0) mbar_arrive_leader(bar); };
       bool edge;
       if constexpr (ADD) {
-        float sum[PER][P::COLS];
+        float x[PER][P::COLS];
 #pragma unroll
         for (int i = 0; i < PER; i++)
 #pragma unroll
-          for (int j = 0; j < P::COLS; j++) sum[i][j] = 0.f;
+          for (int j = 0; j < P::COLS; j++) x[i][j] = 0.f;
 #pragma unroll 1
         for (int u = 0; u < units; u++, local++) {
           if (!arrived(edge)) { ok = false; break; }
           if (mine) {
 #pragma unroll
-            for (int i = 0; i < PER; i++) {
+            for (int i = 0; i < PER; i++)
 #pragma unroll
               for (int q = 0; q < P::COLS / 16; q++) {     // few columns at a time: the sums leave few registers
                 uint32_t r[16];
                 tmem_ld_32x16(lanes + (local & 1) * ACC + (half ? PIECES - 1 - i : i) * P::COLS + 16 * q, r);
                 tmem_ld_wait();
 #pragma unroll
-                for (int j = 0; j < 16; j++) sum[i][16 * q + j] += __uint_as_float(r[j]);
+                for (int j = 0; j < 16; j++) x[i][16 * q + j] += __uint_as_float(r[j]);
               }
-              if (i == 0 && edge) taken(&tmem_empty[0]);
-            }
           }
-          if (!OVERLAP) taken(&tmem_empty[local & 1]);
+          taken(&tmem_empty[local & 1]);
         }
         if (ok && mine) {
 #pragma unroll
-          for (int i = 0; i < PER; i++) ship(sum[i], half ? PIECES - 1 - i : i);
+          for (int i = 0; i < PER; i++) ship(x[i], half ? PIECES - 1 - i : i);
         }
       } else {
         if (!arrived(edge)) { ok = false; break; }
@@ -279,15 +289,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FP8_THREADS, 1) fp8_
           for (int i = 0; i < PER; i++) {
             const int pc = half ? PIECES - 1 - i : i;
             float x[P::COLS];
-#pragma unroll
-            for (int q = 0; q < P::COLS / 32; q++) {
-              uint32_t r[32];
-              tmem_ld_32x32(lanes + (local & 1) * ACC + pc * P::COLS + 32 * q, r);
-              tmem_ld_wait();
-#pragma unroll
-              for (int j = 0; j < 32; j++) x[32 * q + j] = __uint_as_float(r[j]);
-            }
-            if (i == 0 && edge) taken(&tmem_empty[0]);
+            auto load = [&](int q) { tmem_ld_32x32(lanes + (local & 1) * ACC + pc * P::COLS + 32 * q, reinterpret_cast<uint32_t (&)[32]>(x[32 * q])); };
+            // the columns that the accumulators share first: the last ones of the upper half, the first ones of the lower
+            if (half) load(1); else load(0);
+            if (i == 0 && edge) { tmem_ld_wait(); taken(&tmem_empty[0]); }
+            if (half) load(0); else load(1);
+            tmem_ld_wait();
             ship(x, pc);
           }
         }
