@@ -17,7 +17,7 @@ struct AdamTensor {
   long long n, block;
   int flags, pad;
 };
-enum { ADAM_DECAY = 1, ADAM_P_F32 = 2, ADAM_G_F32 = 4, ADAM_WORDS = 8 };      // WORDS: every address on a boundary of four elements
+enum { ADAM_DECAY = 1, ADAM_P_F32 = 2, ADAM_G_F32 = 4, ADAM_WORDS = 8 };      // WORDS: every address on a boundary of 16 bytes
 
 struct AdamArgs {
   const AdamTensor* tensors; int count; long long blocks;
@@ -33,36 +33,117 @@ __device__ __forceinline__ uint32_t random_bits(uint32_t place, uint32_t key) {
   h = (h ^ (h >> 15)) * 0x6A09E667u;
   return h ^ (h >> 16);
 }
-__device__ __forceinline__ void e4m3_values(uint32_t four, float (&v)[4]) {
+__device__ __forceinline__ void e4m3_values(uint32_t four, float f, f32x2 (&v)[2]) {      // times f
 #pragma unroll
   for (int i = 0; i < 2; i++) {
     const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(four >> (16 * i)), __NV_E4M3);
-    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
-    v[2 * i] = f.x; v[2 * i + 1] = f.y;
+    const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&h));
+    v[i] = mul2(pack2(x.x, x.y), both2(f));
   }
 }
-// x / scale rounded to e4m3, up with probability (part cut off) * 2^16 of bits 0..15 of `bits`
-template <bool POSITIVE> __device__ __forceinline__ float stochastic(float x, float f, uint32_t bits) {
-  const float t = x * f, a = fabsf(t), low = a < 0.015625f ? 0.015625f : 0.f;      // below 2^-6 the steps are those of [2^-6, 2^-5)
-  float z = __uint_as_float((__float_as_uint(a + low) + (bits << 4)) & 0xfff00000u) - low;
+// t, at most 448 in magnitude, rounded to a value of e4m3: up if the part cut off and 16 random bits (times 2^4) carry
+template <bool POSITIVE> __device__ __forceinline__ float stochastic(float t, uint32_t bits) {
+  const float a = fabsf(t), low = a < 0.015625f ? 0.015625f : 0.f;      // below 2^-6 the steps are those of [2^-6, 2^-5)
+  float z = __uint_as_float((__float_as_uint(a + low) + bits) & 0xfff00000u) - low;
   if (POSITIVE && a > 0.f) z = fmaxf(z, 0.001953125f);
-  return finite_bits(x) | (x == 0.f) ? copysignf(z, t) : __uint_as_float(0x7fffffffu);
+  return POSITIVE ? z : copysignf(z, t);
 }
-template <bool POSITIVE> __device__ __forceinline__ uint32_t round_block(const float (&x)[4], const uint32_t (&bits)[4], uint32_t& byte) {
+// Eight of a block's values, by 16 lanes -> their bytes and the block's
+template <bool POSITIVE> __device__ __forceinline__ uint2 round_block(f32x2 (&x2)[4], const uint32_t (&random)[8], uint32_t mask, uint32_t& byte) {
+  float x[8];
+#pragma unroll
+  for (int i = 0; i < 4; i++) unpack2(x2[i], x[2 * i], x[2 * i + 1]);
   uint32_t top = 0;
 #pragma unroll
-  for (int e = 0; e < 4; e++) top = max(top, finite_bits(x[e]));
-  byte = scale_byte(__reduce_max_sync(0xffffffffu, top));
-  const float f = scale_inverse(byte);
-  float z[4];
+  for (int e = 0; e < 8; e++) top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
+  const bool odd = __any_sync(mask, top >= kInf);
+  if (odd) {
+    top = 0;
 #pragma unroll
-  for (int e = 0; e < 4; e++) z[e] = stochastic<POSITIVE>(x[e], f, POSITIVE ? bits[e] >> 16 : bits[e] & 0xffffu);
-  return e4m3_pair(z[0], z[1]) | e4m3_pair(z[2], z[3]) << 16;
+    for (int e = 0; e < 8; e++) top = max(top, finite_bits(x[e]));
+  }
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(mask, top, o));
+  byte = scale_byte(top);
+  const f32x2 f = both2(scale_inverse(byte));
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    float t[2];
+    unpack2(mul2(x2[i], f), t[0], t[1]);
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      const uint32_t r = random[2 * i + h];
+      const float z = stochastic<POSITIVE>(t[h], POSITIVE ? (r >> 12) & 0xffff0u : (r << 4) & 0xffff0u);
+      x[2 * i + h] = odd ? nan_or(x[2 * i + h], z) : z;
+    }
+  }
+  return make_uint2(e4m3_pair(x[0], x[1]) | e4m3_pair(x[2], x[3]) << 16, e4m3_pair(x[4], x[5]) | e4m3_pair(x[6], x[7]) << 16);
 }
 
-// A warp has a block of 128 elements, a lane four of them.
+// Eight elements of a lane as they come from memory
+template <bool BITS8> struct AdamRaw {
+  static constexpr int S = BITS8 ? 2 : 8;                  // words of a moment
+  uint32_t g[8], w[8], m[S], v[S];
+  uint32_t fm, fv;                                         // bytes of the moments' scales
+};
+// Where a block lies
+struct AdamPlace {
+  void* p; float* master; const void* g;
+  long long i;                                             // first element of the lane
+  int left, flags;                                         // elements of the lane, at most 8 (not positive: none)
+  __device__ __forceinline__ bool words() const { return (flags & ADAM_WORDS) && left == 8; }
+};
+__device__ __forceinline__ void load_words(const void* p, uint32_t (&w)[8]) {
+  const uint4 a = static_cast<const uint4*>(p)[0], b = static_cast<const uint4*>(p)[1];
+  w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w; w[4] = b.x; w[5] = b.y; w[6] = b.z; w[7] = b.w;
+}
+__device__ __forceinline__ void load_words(const void* p, uint32_t (&w)[2]) { const uint2 a = *static_cast<const uint2*>(p); w[0] = a.x; w[1] = a.y; }
+__device__ __forceinline__ void store_words(void* p, const uint32_t (&w)[8]) {
+  static_cast<uint4*>(p)[0] = make_uint4(w[0], w[1], w[2], w[3]); static_cast<uint4*>(p)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+}
+
+__device__ __forceinline__ AdamPlace adam_place(const AdamArgs& a, long long block, int l16, int& at) {
+  if (at + 1 < a.count && a.tensors[at + 1].block <= block) {           // the last tensor that begins at or before the block
+    int lo = at + 1, hi = a.count;
+    while (hi - lo > 1) { const int mid = (lo + hi) / 2; (a.tensors[mid].block <= block ? lo : hi) = mid; }
+    at = lo;
+  }
+  const AdamTensor& q = a.tensors[at];
+  AdamPlace o;
+  o.flags = q.flags; o.p = q.p; o.master = o.flags & ADAM_P_F32 ? static_cast<float*>(q.p) : q.master; o.g = q.g;
+  o.i = (block - q.block) * 128 + l16 * 8;
+  o.left = (int)min(8ll, q.n - o.i);
+  return o;
+}
+template <bool BITS8> __device__ __forceinline__ void adam_load(const AdamArgs& a, const AdamPlace& o, long long block, int l16, AdamRaw<BITS8>& r) {
+  if (o.words()) {
+    if (o.flags & ADAM_G_F32) load_words(static_cast<const float*>(o.g) + o.i, r.g);
+    else { const uint4 u = *reinterpret_cast<const uint4*>(static_cast<const bf16*>(o.g) + o.i); r.g[0] = u.x; r.g[1] = u.y; r.g[2] = u.z; r.g[3] = u.w; }
+    load_words(o.master + o.i, r.w);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; e++) { r.g[e] = 0; r.w[e] = 0; }
+#pragma unroll
+    for (int e = 0; e < 8; e++) if (e < o.left) {
+      if (o.flags & ADAM_G_F32) r.g[e] = static_cast<const uint32_t*>(o.g)[o.i + e];
+      else r.g[e >> 1] |= (uint32_t)static_cast<const uint16_t*>(o.g)[o.i + e] << (16 * (e & 1));
+      r.w[e] = __float_as_uint(o.master[o.i + e]);
+    }
+  }
+  const long long s = block * 128 + l16 * 8;
+  if (BITS8) {
+    load_words(static_cast<const uint8_t*>(a.m) + s, r.m);
+    load_words(static_cast<const uint8_t*>(a.v) + s, r.v);
+    r.fm = a.ms[block]; r.fv = a.vs[block];
+  } else {
+    load_words(static_cast<const float*>(a.m) + s, r.m);
+    load_words(static_cast<const float*>(a.v) + s, r.v);
+  }
+}
+
+// Sixteen lanes have a block of 128 elements, a lane eight of them; the next block's are on their way while one is worked on.
 template <bool BITS8>
-__global__ void __launch_bounds__(256) adamw_many_kernel(const AdamArgs a) {
+__global__ void __launch_bounds__(256, BITS8 ? 3 : 2) adamw_many_kernel(const AdamArgs a) {
   pdl_begin();
   __shared__ float s_c[2];
   const int t = *(volatile int*)a.step + 1;
@@ -71,84 +152,82 @@ __global__ void __launch_bounds__(256) adamw_many_kernel(const AdamArgs a) {
     s_c[1] = (float)(1.0 / sqrt(-expm1(t * a.lb2)));
   }
   __syncthreads();
-  const float rc1 = s_c[0], rc2 = s_c[1], gscale = a.gscale_dev ? a.gscale * *a.gscale_dev : a.gscale;
-  const uint32_t key = a.seed + (uint32_t)t * 0x9E3779B9u;
-  const int lane = threadIdx.x & 31;
-  const long long stride = gridDim.x * 8ll;
+  const float rc2 = s_c[1], gscale = a.gscale_dev ? a.gscale * *a.gscale_dev : a.gscale, lr1 = a.lr * s_c[0];
+  const uint32_t key = a.seed + (uint32_t)t * 0x9E3779B9u, mask = 0xffffu << (threadIdx.x & 16);
+  const int l16 = threadIdx.x & 15;
+  const long long stride = gridDim.x * 16ll;
+  long long block = blockIdx.x * 16ll + (threadIdx.x >> 4);
   int at = 0;
-  for (long long block = blockIdx.x * 8ll + (threadIdx.x >> 5); block < a.blocks; block += stride) {
-    if (at + 1 < a.count && a.tensors[at + 1].block <= block) {      // the last tensor that begins at or before the block
-      int lo = at + 1, hi = a.count;
-      while (hi - lo > 1) { const int mid = (lo + hi) / 2; (a.tensors[mid].block <= block ? lo : hi) = mid; }
-      at = lo;
-    }
-    const AdamTensor& q = a.tensors[at];
-    const int flags = q.flags;
-    const long long i = (block - q.block) * 128 + lane * 4, s = block * 128 + lane * 4;
-    const int left = (int)min(4ll, q.n - i);                          // elements of this lane, none or fewer if not positive
-    const bool words = (flags & ADAM_WORDS) && left == 4;
-    float g[4] = {0.f, 0.f, 0.f, 0.f}, w[4] = {0.f, 0.f, 0.f, 0.f}, m[4], v[4];
-    float* const master = flags & ADAM_P_F32 ? static_cast<float*>(q.p) : q.master;
-    if (words) {
-      if (flags & ADAM_G_F32) *reinterpret_cast<float4*>(g) = reinterpret_cast<const float4*>(static_cast<const float*>(q.g) + i)[0];
-      else {
-        const uint2 u = *reinterpret_cast<const uint2*>(static_cast<const bf16*>(q.g) + i);
-        g[0] = __uint_as_float(u.x << 16); g[1] = __uint_as_float(u.x & 0xffff0000u); g[2] = __uint_as_float(u.y << 16); g[3] = __uint_as_float(u.y & 0xffff0000u);
-      }
-      *reinterpret_cast<float4*>(w) = *reinterpret_cast<const float4*>(master + i);
-    } else {
+  AdamRaw<BITS8> r, next;
+  AdamPlace o, then;
+  if (block < a.blocks) { o = adam_place(a, block, l16, at); adam_load(a, o, block, l16, r); }
+  for (; block < a.blocks; block += stride, o = then, r = next) {
+    if (block + stride < a.blocks) { then = adam_place(a, block + stride, l16, at); adam_load(a, then, block + stride, l16, next); }
+    f32x2 g[4], m[4], v[4], root[4];
+    float w[8];
 #pragma unroll
-      for (int e = 0; e < 4; e++) if (e < left) {
-        g[e] = flags & ADAM_G_F32 ? static_cast<const float*>(q.g)[i + e] : __bfloat162float(static_cast<const bf16*>(q.g)[i + e]);
-        w[e] = master[i + e];
-      }
+    for (int i = 0; i < 4; i++) {
+      g[i] = o.flags & ADAM_G_F32 ? pack2(__uint_as_float(r.g[2 * i]), __uint_as_float(r.g[2 * i + 1])) : pack2(__uint_as_float(r.g[i] << 16), __uint_as_float(r.g[i] & 0xffff0000u));
+      g[i] = mul2(g[i], both2(gscale));
     }
     if (BITS8) {
-      e4m3_values(static_cast<const uint32_t*>(a.m)[s / 4], m);
-      e4m3_values(static_cast<const uint32_t*>(a.v)[s / 4], v);
-      const float fm = scale_value(a.ms[block]), fv = scale_value(a.vs[block]);
+      const float fm = scale_value(r.fm), fv = scale_value(r.fv);
 #pragma unroll
-      for (int e = 0; e < 4; e++) { m[e] *= fm; v[e] *= fv; v[e] = __fmul_rn(v[e], v[e]); }
-    } else {
-      *reinterpret_cast<float4*>(m) = *reinterpret_cast<const float4*>(static_cast<const float*>(a.m) + s);
-      *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(static_cast<const float*>(a.v) + s);
-    }
-    const float keep = 1.f - a.lr * (flags & ADAM_DECAY ? a.wd : 0.f);
-    float r[4];
-#pragma unroll
-    for (int e = 0; e < 4; e++) {
-      const float x = __fmul_rn(g[e], gscale);
-      m[e] = __fadd_rn(__fmul_rn(a.b1, m[e]), __fmul_rn(a.c1, x));
-      v[e] = __fadd_rn(__fmul_rn(a.b2, v[e]), __fmul_rn(__fmul_rn(a.c2, x), x));
-      r[e] = __fsqrt_rn(v[e]);
-      w[e] = w[e] * keep - a.lr * (m[e] * rc1) / (r[e] * rc2 + a.eps);
-    }
-    if (words) {
-      *reinterpret_cast<float4*>(master + i) = *reinterpret_cast<const float4*>(w);
-      if (!(flags & ADAM_P_F32)) {
-        __nv_bfloat162 o[2] = {__floats2bfloat162_rn(w[0], w[1]), __floats2bfloat162_rn(w[2], w[3])};
-        *reinterpret_cast<uint2*>(static_cast<bf16*>(q.p) + i) = *reinterpret_cast<const uint2*>(o);
+      for (int i = 0; i < 2; i++) {
+        e4m3_values(r.m[i], fm, reinterpret_cast<f32x2 (&)[2]>(m[2 * i]));
+        e4m3_values(r.v[i], fv, reinterpret_cast<f32x2 (&)[2]>(v[2 * i]));
       }
+#pragma unroll
+      for (int i = 0; i < 4; i++) v[i] = mul2(v[i], v[i]);
     } else {
 #pragma unroll
-      for (int e = 0; e < 4; e++) if (e < left) {
-        master[i + e] = w[e];
-        if (!(flags & ADAM_P_F32)) static_cast<bf16*>(q.p)[i + e] = __float2bfloat16_rn(w[e]);
+      for (int i = 0; i < 4; i++) {
+        m[i] = pack2(__uint_as_float(r.m[2 * i]), __uint_as_float(r.m[2 * i + 1]));
+        v[i] = pack2(__uint_as_float(r.v[2 * i]), __uint_as_float(r.v[2 * i + 1]));
       }
     }
+    const float keep = 1.f - a.lr * (o.flags & ADAM_DECAY ? a.wd : 0.f);
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      m[i] = add2(mul2(both2(a.b1), m[i]), mul2(both2(a.c1), g[i]));
+      v[i] = add2(mul2(both2(a.b2), v[i]), mul2(mul2(both2(a.c2), g[i]), g[i]));
+      float x, y, d, e; unpack2(v[i], x, y);
+      x = __fsqrt_rn(x); y = __fsqrt_rn(y);
+      root[i] = pack2(x, y);
+      unpack2(fma2(root[i], both2(rc2), both2(a.eps)), d, e);
+      unpack2(mul2(m[i], both2(lr1)), x, y);
+      w[2 * i] = fmaf(__uint_as_float(r.w[2 * i]), keep, -__fdividef(x, d));
+      w[2 * i + 1] = fmaf(__uint_as_float(r.w[2 * i + 1]), keep, -__fdividef(y, e));
+    }
+    if (o.words()) {
+      store_words(o.master + o.i, reinterpret_cast<const uint32_t (&)[8]>(w));
+      if (!(o.flags & ADAM_P_F32)) *reinterpret_cast<bf16x8*>(static_cast<bf16*>(o.p) + o.i) = pack8(w);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; e++) if (e < o.left) {
+        o.master[o.i + e] = w[e];
+        if (!(o.flags & ADAM_P_F32)) static_cast<bf16*>(o.p)[o.i + e] = __float2bfloat16_rn(w[e]);
+      }
+    }
+    const long long s = block * 128 + l16 * 8;
     if (BITS8) {
-      uint32_t bits[4], bm, bv;
+      uint32_t random[8], bm, bv;
 #pragma unroll
-      for (int e = 0; e < 4; e++) bits[e] = random_bits((uint32_t)s + e, key);
+      for (int e = 0; e < 8; e++) random[e] = random_bits((uint32_t)s + e, key);
+      if (o.left < 8) {                                     // what lies beyond the tensor stays zero
 #pragma unroll
-      for (int e = 0; e < 4; e++) if (e >= left) { m[e] = 0.f; r[e] = 0.f; }
-      const uint32_t om = round_block<false>(m, bits, bm), ov = round_block<true>(r, bits, bv);
-      static_cast<uint32_t*>(a.m)[s / 4] = om;
-      static_cast<uint32_t*>(a.v)[s / 4] = ov;
-      if (lane == 0) { a.ms[block] = bm; a.vs[block] = bv; }
+        for (int i = 0; i < 4; i++) {
+          float x, y;
+          unpack2(m[i], x, y); m[i] = pack2(2 * i < o.left ? x : 0.f, 2 * i + 1 < o.left ? y : 0.f);
+          unpack2(root[i], x, y); root[i] = pack2(2 * i < o.left ? x : 0.f, 2 * i + 1 < o.left ? y : 0.f);
+        }
+      }
+      *reinterpret_cast<uint2*>(static_cast<uint8_t*>(a.m) + s) = round_block<false>(m, random, mask, bm);
+      *reinterpret_cast<uint2*>(static_cast<uint8_t*>(a.v) + s) = round_block<true>(root, random, mask, bv);
+      if (l16 == 0) { a.ms[block] = bm; a.vs[block] = bv; }
     } else {
-      *reinterpret_cast<float4*>(static_cast<float*>(a.m) + s) = *reinterpret_cast<const float4*>(m);
-      *reinterpret_cast<float4*>(static_cast<float*>(a.v) + s) = *reinterpret_cast<const float4*>(v);
+      store_words(static_cast<float*>(a.m) + s, reinterpret_cast<const uint32_t (&)[8]>(m));
+      store_words(static_cast<float*>(a.v) + s, reinterpret_cast<const uint32_t (&)[8]>(v));
     }
   }
   __syncthreads();                                        // every thread has read *step
@@ -170,7 +249,7 @@ int piccl_ops_adamw_many(const void* tensors, int count, long long blocks, int b
   if ((reinterpret_cast<uintptr_t>(m) | reinterpret_cast<uintptr_t>(v)) & 15) return -2;
   AdamArgs a{static_cast<const AdamTensor*>(tensors), count, blocks, m, v, (uint8_t*)ms, (uint8_t*)vs, lr, (float)b1, (float)(1 - b1), (float)b2, (float)(1 - b2), eps, wd, log(b1), log(b2),
              gscale, gscale_dev, step, ticket, seed};
-  const long long want = (blocks + 7) / 8, most = 148 * 8;
+  const long long want = (blocks + 15) / 16, most = 148 * (bits8 ? 3 : 2);
   const unsigned grid = (unsigned)(want < 1 ? 1 : want < most ? want : most);
   const cudaError_t e = launch_pdl(bits8 ? adamw_many_kernel<true> : adamw_many_kernel<false>, dim3(grid), 256, 0, (cudaStream_t)stream, a);
   return e == cudaSuccess ? 0 : (int)e;

@@ -75,6 +75,7 @@ template <typename T> __device__ __forceinline__ uint32_t finite_top8(const Eigh
 }
 // satfinite takes infinities for 448: they are turned into NaN before, where there are any
 __device__ __forceinline__ float nan_of_inf(float x) { return (__float_as_uint(x) & 0x7fffffffu) >= kInf ? __uint_as_float(0x7fffffffu) : x; }
+__device__ __forceinline__ float nan_or(float x, float z) { return (__float_as_uint(x) & 0x7fffffffu) >= kInf ? __uint_as_float(0x7fffffffu) : z; }
 __device__ __forceinline__ uint32_t pack4(float a, float b, float c, float d, float f) {
   float x, y, z, w;
   unpack2(mul2(pack2(a, b), both2(f)), x, y);
