@@ -41,43 +41,58 @@ __device__ __forceinline__ void e4m3_values(uint32_t four, float f, f32x2 (&v)[2
     v[i] = mul2(pack2(x.x, x.y), both2(f));
   }
 }
-// t, at most 448 in magnitude, rounded to a value of e4m3: up if the part cut off and 16 random bits (times 2^4) carry
-template <bool POSITIVE> __device__ __forceinline__ float stochastic(float t, uint32_t bits) {
+__device__ __forceinline__ float max3_nan(float a, float b, float c) { float r; asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c)); return r; }
+__device__ __forceinline__ float min3(float a, float b, float c) { float r; asm("min.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c)); return r; }
+// Where an element's 16 random bits stand among the 20 that are cut off
+template <bool ROOT> __device__ __forceinline__ uint32_t random_part(uint32_t r) { return (ROOT ? r >> 16 : r & 0xffffu) << 4; }
+// x / scale, at most 448 in magnitude, rounded: what is cut off of its fraction, and the random bits, carry.  Its magnitude is 2^-6 or more: the steps of e4m3 are those of three bits of fraction.
+template <bool ROOT> __device__ __forceinline__ float stochastic(float t, uint32_t r) { return __uint_as_float((__float_as_uint(t) + random_part<ROOT>(r)) & 0xfff00000u); }
+// The same for any magnitude, and NaN for x that is not finite; a root that is not zero stays so
+template <bool ROOT> __device__ __forceinline__ float stochastic_any(float x, float t, uint32_t r) {
+  if ((__float_as_uint(x) & 0x7fffffffu) >= kInf) return __uint_as_float(0x7fffffffu);
   const float a = fabsf(t), low = a < 0.015625f ? 0.015625f : 0.f;      // below 2^-6 the steps are those of [2^-6, 2^-5)
-  float z = __uint_as_float((__float_as_uint(a + low) + bits) & 0xfff00000u) - low;
-  if (POSITIVE && a > 0.f) z = fmaxf(z, 0.001953125f);
-  return POSITIVE ? z : copysignf(z, t);
+  float z = stochastic<ROOT>(a + low, r) - low;
+  if (ROOT && a > 0.f) z = fmaxf(z, 0.001953125f);
+  return copysignf(z, t);
 }
-// Eight of a block's values, by 16 lanes -> their bytes and the block's
-template <bool POSITIVE> __device__ __forceinline__ uint2 round_block(f32x2 (&x2)[4], const uint32_t (&random)[8], uint32_t mask, uint32_t& byte) {
-  float x[8];
+// The byte of a block whose largest value is the root of v: the smallest s for which v <= (448 * 2^s)^2 = 1.53125 * 2^(17 + 2 s).  (A root rounded to fp32 is above 448 * 2^s exactly
+// where v is above that, so this is the byte of correctly rounded roots.)
+__device__ __forceinline__ uint32_t scale_byte_of_root(uint32_t v_bits) {
+  const int e = (int)((v_bits + (0x7fffffu - 0x440000u)) >> 23) - 127 - 17, s = 127 + ((e + 1) >> 1);
+  return v_bits < 0x00800000u ? 1u : (uint32_t)s;
+}
+// Eight of a block's values, by 16 lanes -> their bytes and the block's; of: what the values are the roots of (the values themselves, if they are not roots)
+template <bool ROOT> __device__ __forceinline__ uint2 round_block(const f32x2 (&x2)[4], const f32x2 (&of)[4], const uint32_t (&random)[8], uint32_t mask, uint32_t& byte) {
+  float x[8], y[8];
 #pragma unroll
-  for (int i = 0; i < 4; i++) unpack2(x2[i], x[2 * i], x[2 * i + 1]);
-  uint32_t top = 0;
+  for (int i = 0; i < 4; i++) { unpack2(x2[i], x[2 * i], x[2 * i + 1]); unpack2(of[i], y[2 * i], y[2 * i + 1]); }
+  float most = max3_nan(fabsf(y[0]), fabsf(y[1]), fabsf(y[2])), least = min3(fabsf(x[0]), fabsf(x[1]), fabsf(x[2]));
 #pragma unroll
-  for (int e = 0; e < 8; e++) top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
-  const bool odd = __any_sync(mask, top >= kInf);
+  for (int e = 3; e < 7; e += 2) { most = max3_nan(most, fabsf(y[e]), fabsf(y[e + 1])); least = min3(least, fabsf(x[e]), fabsf(x[e + 1])); }
+  most = max3_nan(most, fabsf(y[7]), fabsf(y[7])); least = fminf(least, fabsf(x[7]));
+  uint32_t top = __float_as_uint(most);
+  bool odd = __any_sync(mask, top >= kInf);
   if (odd) {
     top = 0;
 #pragma unroll
-    for (int e = 0; e < 8; e++) top = max(top, finite_bits(x[e]));
+    for (int e = 0; e < 8; e++) top = max(top, finite_bits(y[e]));
   }
 #pragma unroll
   for (int o = 8; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(mask, top, o));
-  byte = scale_byte(top);
-  const f32x2 f = both2(scale_inverse(byte));
+  byte = ROOT ? scale_byte_of_root(top) : scale_byte(top);
+  const float f = scale_inverse(byte);
+  odd = odd || __any_sync(mask, least * f < 0.015625f);
+  float t[8];
 #pragma unroll
-  for (int i = 0; i < 4; i++) {
-    float t[2];
-    unpack2(mul2(x2[i], f), t[0], t[1]);
+  for (int i = 0; i < 4; i++) unpack2(mul2(x2[i], both2(f)), t[2 * i], t[2 * i + 1]);
+  if (odd) {
 #pragma unroll
-    for (int h = 0; h < 2; h++) {
-      const uint32_t r = random[2 * i + h];
-      const float z = stochastic<POSITIVE>(t[h], POSITIVE ? (r >> 12) & 0xffff0u : (r << 4) & 0xffff0u);
-      x[2 * i + h] = odd ? nan_or(x[2 * i + h], z) : z;
-    }
+    for (int e = 0; e < 8; e++) t[e] = stochastic_any<ROOT>(x[e], t[e], random[e]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; e++) t[e] = stochastic<ROOT>(t[e], random[e]);
   }
-  return make_uint2(e4m3_pair(x[0], x[1]) | e4m3_pair(x[2], x[3]) << 16, e4m3_pair(x[4], x[5]) | e4m3_pair(x[6], x[7]) << 16);
+  return make_uint2(e4m3_pair(t[0], t[1]) | e4m3_pair(t[2], t[3]) << 16, e4m3_pair(t[4], t[5]) | e4m3_pair(t[6], t[7]) << 16);
 }
 
 // Eight elements of a lane as they come from memory
@@ -86,10 +101,15 @@ template <bool BITS8> struct AdamRaw {
   uint32_t g[8], w[8], m[S], v[S];
   uint32_t fm, fv;                                         // bytes of the moments' scales
 };
-// Where a block lies
-struct AdamPlace {
+// The tensor that a lane works on
+struct AdamNow {
   void* p; float* master; const void* g;
-  long long i;                                             // first element of the lane
+  long long n, first, end;                                 // elements; its first block, that of the next tensor
+  int at, flags;
+};
+// Where eight elements of it lie
+struct AdamPlace {
+  float* master; bf16* p;                                  // p: null if the parameters are the masters
   int left, flags;                                         // elements of the lane, at most 8 (not positive: none)
   __device__ __forceinline__ bool words() const { return (flags & ADAM_WORDS) && left == 8; }
 };
@@ -102,32 +122,29 @@ __device__ __forceinline__ void store_words(void* p, const uint32_t (&w)[8]) {
   static_cast<uint4*>(p)[0] = make_uint4(w[0], w[1], w[2], w[3]); static_cast<uint4*>(p)[1] = make_uint4(w[4], w[5], w[6], w[7]);
 }
 
-__device__ __forceinline__ AdamPlace adam_place(const AdamArgs& a, long long block, int l16, int& at) {
-  if (at + 1 < a.count && a.tensors[at + 1].block <= block) {           // the last tensor that begins at or before the block
-    int lo = at + 1, hi = a.count;
-    while (hi - lo > 1) { const int mid = (lo + hi) / 2; (a.tensors[mid].block <= block ? lo : hi) = mid; }
-    at = lo;
-  }
-  const AdamTensor& q = a.tensors[at];
-  AdamPlace o;
-  o.flags = q.flags; o.p = q.p; o.master = o.flags & ADAM_P_F32 ? static_cast<float*>(q.p) : q.master; o.g = q.g;
-  o.i = (block - q.block) * 128 + l16 * 8;
-  o.left = (int)min(8ll, q.n - o.i);
-  return o;
+__device__ __forceinline__ void adam_find(const AdamArgs& a, long long block, AdamNow& c) {      // the last tensor that begins at or before the block, from c.at on
+  int lo = c.at, hi = a.count;
+  while (hi - lo > 1) { const int mid = (lo + hi) / 2; (a.tensors[mid].block <= block ? lo : hi) = mid; }
+  const AdamTensor& q = a.tensors[lo];
+  c.at = lo; c.flags = q.flags; c.p = q.flags & ADAM_P_F32 ? nullptr : q.p; c.master = q.flags & ADAM_P_F32 ? static_cast<float*>(q.p) : q.master; c.g = q.g; c.n = q.n; c.first = q.block;
+  c.end = lo + 1 < a.count ? a.tensors[lo + 1].block : a.blocks;
 }
-template <bool BITS8> __device__ __forceinline__ void adam_load(const AdamArgs& a, const AdamPlace& o, long long block, int l16, AdamRaw<BITS8>& r) {
+template <bool BITS8> __device__ __forceinline__ AdamPlace adam_load(const AdamArgs& a, AdamNow& c, long long block, int l16, AdamRaw<BITS8>& r) {
+  if (block >= c.end) adam_find(a, block, c);
+  const long long i = (block - c.first) * 128 + l16 * 8;
+  AdamPlace o{c.master + i, c.p ? static_cast<bf16*>(c.p) + i : nullptr, (int)min(8ll, c.n - i), c.flags};
   if (o.words()) {
-    if (o.flags & ADAM_G_F32) load_words(static_cast<const float*>(o.g) + o.i, r.g);
-    else { const uint4 u = *reinterpret_cast<const uint4*>(static_cast<const bf16*>(o.g) + o.i); r.g[0] = u.x; r.g[1] = u.y; r.g[2] = u.z; r.g[3] = u.w; }
-    load_words(o.master + o.i, r.w);
+    if (o.flags & ADAM_G_F32) load_words(static_cast<const float*>(c.g) + i, r.g);
+    else { const uint4 u = *reinterpret_cast<const uint4*>(static_cast<const bf16*>(c.g) + i); r.g[0] = u.x; r.g[1] = u.y; r.g[2] = u.z; r.g[3] = u.w; }
+    load_words(o.master, r.w);
   } else {
 #pragma unroll
     for (int e = 0; e < 8; e++) { r.g[e] = 0; r.w[e] = 0; }
 #pragma unroll
     for (int e = 0; e < 8; e++) if (e < o.left) {
-      if (o.flags & ADAM_G_F32) r.g[e] = static_cast<const uint32_t*>(o.g)[o.i + e];
-      else r.g[e >> 1] |= (uint32_t)static_cast<const uint16_t*>(o.g)[o.i + e] << (16 * (e & 1));
-      r.w[e] = __float_as_uint(o.master[o.i + e]);
+      if (o.flags & ADAM_G_F32) r.g[e] = static_cast<const uint32_t*>(c.g)[i + e];
+      else r.g[e >> 1] |= (uint32_t)static_cast<const uint16_t*>(c.g)[i + e] << (16 * (e & 1));
+      r.w[e] = __float_as_uint(o.master[e]);
     }
   }
   const long long s = block * 128 + l16 * 8;
@@ -139,6 +156,13 @@ template <bool BITS8> __device__ __forceinline__ void adam_load(const AdamArgs& 
     load_words(static_cast<const float*>(a.m) + s, r.m);
     load_words(static_cast<const float*>(a.v) + s, r.v);
   }
+  return o;
+}
+// The root of v: in 8 bits the approximate one (2^-23; what it is rounded to has 2^-4), in which v below 2^-126 counts as zero
+template <bool BITS8> __device__ __forceinline__ float adam_root(float v) {
+  float r;
+  if (BITS8) asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v)); else r = __fsqrt_rn(v);
+  return r;
 }
 
 // Sixteen lanes have a block of 128 elements, a lane eight of them; the next block's are on their way while one is worked on.
@@ -157,12 +181,13 @@ __global__ void __launch_bounds__(256, BITS8 ? 3 : 2) adamw_many_kernel(const Ad
   const int l16 = threadIdx.x & 15;
   const long long stride = gridDim.x * 16ll;
   long long block = blockIdx.x * 16ll + (threadIdx.x >> 4);
-  int at = 0;
+  AdamNow now;
+  now.at = 0; now.end = -1;
   AdamRaw<BITS8> r, next;
   AdamPlace o, then;
-  if (block < a.blocks) { o = adam_place(a, block, l16, at); adam_load(a, o, block, l16, r); }
+  if (block < a.blocks) o = adam_load(a, now, block, l16, r);
   for (; block < a.blocks; block += stride, o = then, r = next) {
-    if (block + stride < a.blocks) { then = adam_place(a, block + stride, l16, at); adam_load(a, then, block + stride, l16, next); }
+    if (block + stride < a.blocks) then = adam_load(a, now, block + stride, l16, next);
     f32x2 g[4], m[4], v[4], root[4];
     float w[8];
 #pragma unroll
@@ -192,7 +217,7 @@ __global__ void __launch_bounds__(256, BITS8 ? 3 : 2) adamw_many_kernel(const Ad
       m[i] = add2(mul2(both2(a.b1), m[i]), mul2(both2(a.c1), g[i]));
       v[i] = add2(mul2(both2(a.b2), v[i]), mul2(mul2(both2(a.c2), g[i]), g[i]));
       float x, y, d, e; unpack2(v[i], x, y);
-      x = __fsqrt_rn(x); y = __fsqrt_rn(y);
+      x = adam_root<BITS8>(x); y = adam_root<BITS8>(y);
       root[i] = pack2(x, y);
       unpack2(fma2(root[i], both2(rc2), both2(a.eps)), d, e);
       unpack2(mul2(m[i], both2(lr1)), x, y);
@@ -200,13 +225,13 @@ __global__ void __launch_bounds__(256, BITS8 ? 3 : 2) adamw_many_kernel(const Ad
       w[2 * i + 1] = fmaf(__uint_as_float(r.w[2 * i + 1]), keep, -__fdividef(y, e));
     }
     if (o.words()) {
-      store_words(o.master + o.i, reinterpret_cast<const uint32_t (&)[8]>(w));
-      if (!(o.flags & ADAM_P_F32)) *reinterpret_cast<bf16x8*>(static_cast<bf16*>(o.p) + o.i) = pack8(w);
+      store_words(o.master, reinterpret_cast<const uint32_t (&)[8]>(w));
+      if (o.p) *reinterpret_cast<bf16x8*>(o.p) = pack8(w);
     } else {
 #pragma unroll
       for (int e = 0; e < 8; e++) if (e < o.left) {
-        o.master[o.i + e] = w[e];
-        if (!(o.flags & ADAM_P_F32)) static_cast<bf16*>(o.p)[o.i + e] = __float2bfloat16_rn(w[e]);
+        o.master[e] = w[e];
+        if (o.p) o.p[e] = __float2bfloat16_rn(w[e]);
       }
     }
     const long long s = block * 128 + l16 * 8;
@@ -220,10 +245,11 @@ __global__ void __launch_bounds__(256, BITS8 ? 3 : 2) adamw_many_kernel(const Ad
           float x, y;
           unpack2(m[i], x, y); m[i] = pack2(2 * i < o.left ? x : 0.f, 2 * i + 1 < o.left ? y : 0.f);
           unpack2(root[i], x, y); root[i] = pack2(2 * i < o.left ? x : 0.f, 2 * i + 1 < o.left ? y : 0.f);
+          unpack2(v[i], x, y); v[i] = pack2(2 * i < o.left ? x : 0.f, 2 * i + 1 < o.left ? y : 0.f);
         }
       }
-      *reinterpret_cast<uint2*>(static_cast<uint8_t*>(a.m) + s) = round_block<false>(m, random, mask, bm);
-      *reinterpret_cast<uint2*>(static_cast<uint8_t*>(a.v) + s) = round_block<true>(root, random, mask, bv);
+      *reinterpret_cast<uint2*>(static_cast<uint8_t*>(a.m) + s) = round_block<false>(m, m, random, mask, bm);
+      *reinterpret_cast<uint2*>(static_cast<uint8_t*>(a.v) + s) = round_block<true>(root, v, random, mask, bv);
       if (l16 == 0) { a.ms[block] = bm; a.vs[block] = bv; }
     } else {
       store_words(static_cast<float*>(a.m) + s, reinterpret_cast<const uint32_t (&)[8]>(m));

@@ -84,10 +84,10 @@ def _bits(n, seed, step):
     return h ^ (h >> 16)
 
 
-def _held(x, u, positive):
-    """(e4m3 values, bytes) of blocks, stochastically rounded, in fp64 from what fp32 arithmetic gave"""
+def _held(x, u, positive, off=0.0):
+    """(e4m3 values, bytes) of blocks, stochastically rounded, in fp64 from what fp32 arithmetic gave (times 1 + off)"""
     byte = _bytes(x)
-    t = x.double() * torch.exp2(127.0 - byte.double())[:, None]
+    t = (x.double() * torch.exp2(127.0 - byte.double())[:, None] * (1 + off)).clamp(max=448.0)
     step = torch.exp2(torch.floor(torch.log2(t.abs().clamp(min=2.0 ** -6))) - 3)
     q = torch.floor(t.abs() / step + u.double() / 65536) * step
     if positive:
@@ -125,7 +125,12 @@ def test_moments_in_8_bits(master, grad, offset):
                 full[:n] = now
                 q, byte = _held(full.view(blocks, 128), r[o:o + blocks * 128].view(blocks, 128), positive)
                 assert torch.equal(scales[o // 128:o // 128 + blocks].int(), byte)
-                assert torch.equal(held[o:o + blocks * 128].double(), q.view(-1))
+                got, same = held[o:o + blocks * 128].double(), False
+                if positive:                        # the root is approximate, to 2^-22 of its value: it may be held as its neighbour within that would be
+                    for off in (-2.0 ** -22, 2.0 ** -22):
+                        same |= got == _held(full.view(blocks, 128), r[o:o + blocks * 128].view(blocks, 128), positive, off)[0].view(-1)
+                same |= got == q.view(-1)
+                assert bool(same.all())
             want = _reference(w, m, v, grads[i], step, True, 0.7, **RATES)
             _near(weights[i], want[0], w, 2, 10 * (want[0] - w.double()).abs())
             if master:
