@@ -79,7 +79,7 @@ class AdamW:
             if n == 0:
                 continue
             flags = _DECAY * d | _P_F32 * (w is None) | _G_F32 * (g.dtype == torch.float32)
-            if all(t is None or t.data_ptr() % 16 == 0 for t in (p, w, g)):
+            if all(t is None or t.data_ptr() % (8 * t.element_size()) == 0 for t in (p, w, g)):
                 flags |= _WORDS
             records.append(_Tensor(p.data_ptr(), 0 if w is None else w.data_ptr(), g.data_ptr(), n, first // 128, flags, 0))
         self.grads, self._count = grads, len(records)

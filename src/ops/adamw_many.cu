@@ -17,7 +17,7 @@ struct AdamTensor {
   long long n, block;
   int flags, pad;
 };
-enum { ADAM_DECAY = 1, ADAM_P_F32 = 2, ADAM_G_F32 = 4, ADAM_WORDS = 8 };      // WORDS: every address on a boundary of 16 bytes
+enum { ADAM_DECAY = 1, ADAM_P_F32 = 2, ADAM_G_F32 = 4, ADAM_WORDS = 8 };      // WORDS: every address on a boundary of eight elements
 
 struct AdamArgs {
   const AdamTensor* tensors; int count; long long blocks;
@@ -61,102 +61,75 @@ __device__ __forceinline__ uint32_t scale_byte_of_root(uint32_t v_bits) {
   const int e = (int)((v_bits + (0x7fffffu - 0x440000u)) >> 23) - 127 - 17, s = 127 + ((e + 1) >> 1);
   return v_bits < 0x00800000u ? 1u : (uint32_t)s;
 }
-// Eight of a block's values, by 16 lanes -> their bytes and the block's; of: what the values are the roots of (the values themselves, if they are not roots)
-template <bool ROOT> __device__ __forceinline__ uint2 round_block(const f32x2 (&x2)[4], const f32x2 (&of)[4], const uint32_t (&random)[8], uint32_t mask, uint32_t& byte) {
-  float x[8], y[8];
-#pragma unroll
-  for (int i = 0; i < 4; i++) { unpack2(x2[i], x[2 * i], x[2 * i + 1]); unpack2(of[i], y[2 * i], y[2 * i + 1]); }
-  float most = max3_nan(fabsf(y[0]), fabsf(y[1]), fabsf(y[2])), least = min3(fabsf(x[0]), fabsf(x[1]), fabsf(x[2]));
-#pragma unroll
-  for (int e = 3; e < 7; e += 2) { most = max3_nan(most, fabsf(y[e]), fabsf(y[e + 1])); least = min3(least, fabsf(x[e]), fabsf(x[e + 1])); }
-  most = max3_nan(most, fabsf(y[7]), fabsf(y[7])); least = fminf(least, fabsf(x[7]));
-  uint32_t top = __float_as_uint(most);
-  bool odd = __any_sync(mask, top >= kInf);
-  if (odd) {
-    top = 0;
-#pragma unroll
-    for (int e = 0; e < 8; e++) top = max(top, finite_bits(y[e]));
-  }
-#pragma unroll
-  for (int o = 8; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(mask, top, o));
-  byte = ROOT ? scale_byte_of_root(top) : scale_byte(top);
-  const float f = scale_inverse(byte);
-  odd = odd || __any_sync(mask, least * f < 0.015625f);
-  float t[8];
-#pragma unroll
-  for (int i = 0; i < 4; i++) unpack2(mul2(x2[i], both2(f)), t[2 * i], t[2 * i + 1]);
-  if (odd) {
-#pragma unroll
-    for (int e = 0; e < 8; e++) t[e] = stochastic_any<ROOT>(x[e], t[e], random[e]);
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; e++) t[e] = stochastic<ROOT>(t[e], random[e]);
-  }
+__device__ __forceinline__ uint2 e4m3_bytes(const float (&t)[8]) {
   return make_uint2(e4m3_pair(t[0], t[1]) | e4m3_pair(t[2], t[3]) << 16, e4m3_pair(t[4], t[5]) | e4m3_pair(t[6], t[7]) << 16);
 }
+// Eight moments and roots of a block, by 16 lanes -> their bytes and the block's two.  All lanes of a warp call it together (votes and shuffles among a part of them cost a barrier each), and both
+// maxima are found side by side: one after the other, each behind its own votes, the latencies of shuffles were a third of the kernel's time.
+__device__ __forceinline__ void round_moments(const f32x2 (&m2)[4], const f32x2 (&v2)[4], const f32x2 (&r2)[4], const uint32_t (&random)[8], uint2& m_out, uint2& v_out, uint32_t& m_byte, uint32_t& v_byte) {
+  float m[8], v[8], r[8];
+#pragma unroll
+  for (int i = 0; i < 4; i++) { unpack2(m2[i], m[2 * i], m[2 * i + 1]); unpack2(v2[i], v[2 * i], v[2 * i + 1]); unpack2(r2[i], r[2 * i], r[2 * i + 1]); }
+  float m_most = fabsf(m[0]), m_least = fabsf(m[0]), v_most = v[0], r_least = r[0];
+#pragma unroll
+  for (int e = 1; e < 8; e += 2) {
+    m_most = max3_nan(m_most, fabsf(m[e]), fabsf(m[(e + 1) % 8])); m_least = min3(m_least, fabsf(m[e]), fabsf(m[(e + 1) % 8]));
+    v_most = max3_nan(v_most, v[e], v[(e + 1) % 8]); r_least = min3(r_least, r[e], r[(e + 1) % 8]);
+  }
+  uint32_t m_top = __float_as_uint(m_most), v_top = __float_as_uint(v_most);
+  bool odd = __any_sync(0xffffffffu, max(m_top, v_top) >= kInf);
+  if (odd) {
+    m_top = v_top = 0;
+#pragma unroll
+    for (int e = 0; e < 8; e++) { m_top = max(m_top, finite_bits(m[e])); v_top = max(v_top, finite_bits(v[e])); }
+  }
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) {
+    const uint32_t x = __shfl_xor_sync(0xffffffffu, m_top, o), y = __shfl_xor_sync(0xffffffffu, v_top, o);
+    m_top = max(m_top, x); v_top = max(v_top, y);
+  }
+  m_byte = scale_byte(m_top); v_byte = scale_byte_of_root(v_top);
+  const float fm = scale_inverse(m_byte), fr = scale_inverse(v_byte);
+  odd = __any_sync(0xffffffffu, odd || fminf(m_least * fm, r_least * fr) < 0.015625f);
+  float a[8], b[8];
+#pragma unroll
+  for (int i = 0; i < 4; i++) { unpack2(mul2(m2[i], both2(fm)), a[2 * i], a[2 * i + 1]); unpack2(mul2(r2[i], both2(fr)), b[2 * i], b[2 * i + 1]); }
+  if (odd) {
+#pragma unroll
+    for (int e = 0; e < 8; e++) { a[e] = stochastic_any<false>(m[e], a[e], random[e]); b[e] = stochastic_any<true>(r[e], b[e], random[e]); }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; e++) { a[e] = stochastic<false>(a[e], random[e]); b[e] = stochastic<true>(b[e], random[e]); }
+  }
+  m_out = e4m3_bytes(a); v_out = e4m3_bytes(b);
+}
 
-// Eight elements of a lane as they come from memory
-template <bool BITS8> struct AdamRaw {
-  static constexpr int S = BITS8 ? 2 : 8;                  // words of a moment
-  uint32_t g[8], w[8], m[S], v[S];
-  uint32_t fm, fv;                                         // bytes of the moments' scales
-};
 // The tensor that a lane works on
 struct AdamNow {
-  void* p; float* master; const void* g;
+  bf16* p; float* master; const void* g;                   // p: null if the parameters are the masters
   long long n, first, end;                                 // elements; its first block, that of the next tensor
   int at, flags;
 };
-// Where eight elements of it lie
-struct AdamPlace {
-  float* master; bf16* p;                                  // p: null if the parameters are the masters
-  int left, flags;                                         // elements of the lane, at most 8 (not positive: none)
-  __device__ __forceinline__ bool words() const { return (flags & ADAM_WORDS) && left == 8; }
-};
-__device__ __forceinline__ void load_words(const void* p, uint32_t (&w)[8]) {
-  const uint4 a = static_cast<const uint4*>(p)[0], b = static_cast<const uint4*>(p)[1];
-  w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w; w[4] = b.x; w[5] = b.y; w[6] = b.z; w[7] = b.w;
+// N words of 4 bytes from N * 4 bytes' boundary on.  Eight of them in one access of 32 bytes: as two of 16 a warp would touch every sector twice.
+template <int N> __device__ __forceinline__ void load_words(const void* p, uint32_t (&w)[N]) {
+  static_assert(N == 2 || N == 4 || N == 8, "");
+  if constexpr (N == 2) { const uint2 a = *static_cast<const uint2*>(p); w[0] = a.x; w[1] = a.y; }
+  else if constexpr (N == 4) { const uint4 a = *static_cast<const uint4*>(p); w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w; }
+  else asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7]) : "l"(p) : "memory");
 }
-__device__ __forceinline__ void load_words(const void* p, uint32_t (&w)[2]) { const uint2 a = *static_cast<const uint2*>(p); w[0] = a.x; w[1] = a.y; }
-__device__ __forceinline__ void store_words(void* p, const uint32_t (&w)[8]) {
-  static_cast<uint4*>(p)[0] = make_uint4(w[0], w[1], w[2], w[3]); static_cast<uint4*>(p)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+template <int N> __device__ __forceinline__ void store_words(void* p, const uint32_t (&w)[N]) {
+  static_assert(N == 2 || N == 4 || N == 8, "");
+  if constexpr (N == 2) *static_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+  else if constexpr (N == 4) *static_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+  else asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");
 }
-
 __device__ __forceinline__ void adam_find(const AdamArgs& a, long long block, AdamNow& c) {      // the last tensor that begins at or before the block, from c.at on
   int lo = c.at, hi = a.count;
   while (hi - lo > 1) { const int mid = (lo + hi) / 2; (a.tensors[mid].block <= block ? lo : hi) = mid; }
   const AdamTensor& q = a.tensors[lo];
-  c.at = lo; c.flags = q.flags; c.p = q.flags & ADAM_P_F32 ? nullptr : q.p; c.master = q.flags & ADAM_P_F32 ? static_cast<float*>(q.p) : q.master; c.g = q.g; c.n = q.n; c.first = q.block;
+  c.at = lo; c.flags = q.flags; c.g = q.g; c.n = q.n; c.first = q.block;
+  c.p = q.flags & ADAM_P_F32 ? nullptr : static_cast<bf16*>(q.p); c.master = q.flags & ADAM_P_F32 ? static_cast<float*>(q.p) : q.master;
   c.end = lo + 1 < a.count ? a.tensors[lo + 1].block : a.blocks;
-}
-template <bool BITS8> __device__ __forceinline__ AdamPlace adam_load(const AdamArgs& a, AdamNow& c, long long block, int l16, AdamRaw<BITS8>& r) {
-  if (block >= c.end) adam_find(a, block, c);
-  const long long i = (block - c.first) * 128 + l16 * 8;
-  AdamPlace o{c.master + i, c.p ? static_cast<bf16*>(c.p) + i : nullptr, (int)min(8ll, c.n - i), c.flags};
-  if (o.words()) {
-    if (o.flags & ADAM_G_F32) load_words(static_cast<const float*>(c.g) + i, r.g);
-    else { const uint4 u = *reinterpret_cast<const uint4*>(static_cast<const bf16*>(c.g) + i); r.g[0] = u.x; r.g[1] = u.y; r.g[2] = u.z; r.g[3] = u.w; }
-    load_words(o.master, r.w);
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; e++) { r.g[e] = 0; r.w[e] = 0; }
-#pragma unroll
-    for (int e = 0; e < 8; e++) if (e < o.left) {
-      if (o.flags & ADAM_G_F32) r.g[e] = static_cast<const uint32_t*>(c.g)[i + e];
-      else r.g[e >> 1] |= (uint32_t)static_cast<const uint16_t*>(c.g)[i + e] << (16 * (e & 1));
-      r.w[e] = __float_as_uint(o.master[e]);
-    }
-  }
-  const long long s = block * 128 + l16 * 8;
-  if (BITS8) {
-    load_words(static_cast<const uint8_t*>(a.m) + s, r.m);
-    load_words(static_cast<const uint8_t*>(a.v) + s, r.v);
-    r.fm = a.ms[block]; r.fv = a.vs[block];
-  } else {
-    load_words(static_cast<const float*>(a.m) + s, r.m);
-    load_words(static_cast<const float*>(a.v) + s, r.v);
-  }
-  return o;
 }
 // The root of v: in 8 bits the approximate one (2^-23; what it is rounded to has 2^-4), in which v below 2^-126 counts as zero
 template <bool BITS8> __device__ __forceinline__ float adam_root(float v) {
@@ -164,100 +137,159 @@ template <bool BITS8> __device__ __forceinline__ float adam_root(float v) {
   if (BITS8) asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v)); else r = __fsqrt_rn(v);
   return r;
 }
+__device__ __forceinline__ float div_approx(float x, float y) { float r; asm("div.approx.ftz.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(y)); return r; }
 
-// Sixteen lanes have a block of 128 elements, a lane eight of them; the next block's are on their way while one is worked on.
-template <bool BITS8>
-__global__ void __launch_bounds__(256, BITS8 ? 3 : 2) adamw_many_kernel(const AdamArgs a) {
-  pdl_begin();
-  __shared__ float s_c[2];
-  const int t = *(volatile int*)a.step + 1;
-  if (threadIdx.x == 0) {
-    s_c[0] = (float)(1.0 / -expm1(t * a.lb1));
-    s_c[1] = (float)(1.0 / sqrt(-expm1(t * a.lb2)));
+// What the step is, for every thread of a block.
+struct AdamStep {
+  float rc2, lr1, gscale; uint32_t key;
+  __device__ __forceinline__ AdamStep(const AdamArgs& a) {
+    __shared__ float s_c[2];
+    const int t = *(volatile int*)a.step + 1;
+    if (threadIdx.x == 0) {
+      s_c[0] = (float)(1.0 / -expm1(t * a.lb1));
+      s_c[1] = (float)(1.0 / sqrt(-expm1(t * a.lb2)));
+    }
+    __syncthreads();
+    rc2 = s_c[1]; lr1 = a.lr * s_c[0];
+    gscale = a.gscale_dev ? a.gscale * *a.gscale_dev : a.gscale;
+    key = a.seed + (uint32_t)t * 0x9E3779B9u;
   }
-  __syncthreads();
-  const float rc2 = s_c[1], gscale = a.gscale_dev ? a.gscale * *a.gscale_dev : a.gscale, lr1 = a.lr * s_c[0];
-  const uint32_t key = a.seed + (uint32_t)t * 0x9E3779B9u, mask = 0xffffu << (threadIdx.x & 16);
-  const int l16 = threadIdx.x & 15;
-  const long long stride = gridDim.x * 16ll;
-  long long block = blockIdx.x * 16ll + (threadIdx.x >> 4);
+  __device__ __forceinline__ static void done(const AdamArgs& a) {
+    __syncthreads();                                       // every thread has read *step
+    if (threadIdx.x == 0 && atomicAdd(a.ticket, 1u) == gridDim.x - 1) { *a.ticket = 0; atomicAdd(a.step, 1); }
+  }
+  // moments, roots and weights of E elements; w: as bits
+  template <bool BITS8, int E> __device__ __forceinline__ void update(const AdamArgs& a, int flags, const uint32_t (&gw)[E], uint32_t (&w)[E], f32x2 (&m)[E / 2], f32x2 (&v)[E / 2], f32x2 (&root)[E / 2]) const {
+    const float keep = 1.f - a.lr * (flags & ADAM_DECAY ? a.wd : 0.f);
+#pragma unroll
+    for (int k = 0; k < E / 2; k++) {
+      f32x2 g = flags & ADAM_G_F32 ? pack2(__uint_as_float(gw[2 * k]), __uint_as_float(gw[2 * k + 1])) : pack2(__uint_as_float(gw[k] << 16), __uint_as_float(gw[k] & 0xffff0000u));
+      g = mul2(g, both2(gscale));
+      m[k] = add2(mul2(both2(a.b1), m[k]), mul2(both2(a.c1), g));
+      v[k] = add2(mul2(both2(a.b2), v[k]), mul2(mul2(both2(a.c2), g), g));
+      float x, y, d, e; unpack2(v[k], x, y);
+      x = adam_root<BITS8>(x); y = adam_root<BITS8>(y);
+      root[k] = pack2(x, y);
+      unpack2(fma2(root[k], both2(rc2), both2(a.eps)), d, e);
+      unpack2(mul2(m[k], both2(lr1)), x, y);
+      w[2 * k] = __float_as_uint(fmaf(__uint_as_float(w[2 * k]), keep, -div_approx(x, d)));
+      w[2 * k + 1] = __float_as_uint(fmaf(__uint_as_float(w[2 * k + 1]), keep, -div_approx(y, e)));
+    }
+  }
+};
+// E gradients (bf16 in pairs) and weights one by one; left: how many there are
+template <int E> __device__ __forceinline__ void load_some(const void* g, const float* master, int left, int flags, uint32_t (&gw)[E], uint32_t (&w)[E]) {
+#pragma unroll
+  for (int e = 0; e < E; e++) { gw[e] = 0; w[e] = 0; }
+#pragma unroll
+  for (int e = 0; e < E; e++) if (e < left) {
+    if (flags & ADAM_G_F32) gw[e] = static_cast<const uint32_t*>(g)[e];
+    else gw[e >> 1] |= (uint32_t)static_cast<const uint16_t*>(g)[e] << (16 * (e & 1));
+    w[e] = __float_as_uint(master[e]);
+  }
+}
+template <int E> __device__ __forceinline__ void store_weights(float* master, bf16* p, int left, bool words, const uint32_t (&w)[E]) {
+  if (words) {
+    store_words(master, w);
+    if (p) {
+      uint32_t o[E / 2];
+#pragma unroll
+      for (int k = 0; k < E / 2; k++) { const __nv_bfloat162 h = __floats2bfloat162_rn(__uint_as_float(w[2 * k]), __uint_as_float(w[2 * k + 1])); o[k] = *reinterpret_cast<const uint32_t*>(&h); }
+      store_words(p, o);
+    }
+  } else
+#pragma unroll
+    for (int e = 0; e < E; e++) if (e < left) {
+      master[e] = __uint_as_float(w[e]);
+      if (p) p[e] = __float2bfloat16_rn(__uint_as_float(w[e]));
+    }
+}
+__device__ __forceinline__ const void* gradients(const AdamNow& c, long long i) { return static_cast<const char*>(c.g) + i * (c.flags & ADAM_G_F32 ? 4 : 2); }
+
+// Moments in fp32: a lane has four elements of a block, a warp the block.  Bound by memory: 28 bytes an element (bf16 parameters and gradients).
+__global__ void __launch_bounds__(256, 5) adamw_many_kernel(const AdamArgs a) {
+  constexpr int E = 4;
+  pdl_begin();
+  const AdamStep step(a);
+  const int l = threadIdx.x & 31;
+  const long long stride = gridDim.x * 8ll;
   AdamNow now;
   now.at = 0; now.end = -1;
-  AdamRaw<BITS8> r, next;
-  AdamPlace o, then;
-  if (block < a.blocks) o = adam_load(a, now, block, l16, r);
-  for (; block < a.blocks; block += stride, o = then, r = next) {
-    if (block + stride < a.blocks) then = adam_load(a, now, block + stride, l16, next);
-    f32x2 g[4], m[4], v[4], root[4];
-    float w[8];
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-      g[i] = o.flags & ADAM_G_F32 ? pack2(__uint_as_float(r.g[2 * i]), __uint_as_float(r.g[2 * i + 1])) : pack2(__uint_as_float(r.g[i] << 16), __uint_as_float(r.g[i] & 0xffff0000u));
-      g[i] = mul2(g[i], both2(gscale));
-    }
-    if (BITS8) {
-      const float fm = scale_value(r.fm), fv = scale_value(r.fv);
-#pragma unroll
-      for (int i = 0; i < 2; i++) {
-        e4m3_values(r.m[i], fm, reinterpret_cast<f32x2 (&)[2]>(m[2 * i]));
-        e4m3_values(r.v[i], fv, reinterpret_cast<f32x2 (&)[2]>(v[2 * i]));
-      }
-#pragma unroll
-      for (int i = 0; i < 4; i++) v[i] = mul2(v[i], v[i]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; i++) {
-        m[i] = pack2(__uint_as_float(r.m[2 * i]), __uint_as_float(r.m[2 * i + 1]));
-        v[i] = pack2(__uint_as_float(r.v[2 * i]), __uint_as_float(r.v[2 * i + 1]));
-      }
-    }
-    const float keep = 1.f - a.lr * (o.flags & ADAM_DECAY ? a.wd : 0.f);
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-      m[i] = add2(mul2(both2(a.b1), m[i]), mul2(both2(a.c1), g[i]));
-      v[i] = add2(mul2(both2(a.b2), v[i]), mul2(mul2(both2(a.c2), g[i]), g[i]));
-      float x, y, d, e; unpack2(v[i], x, y);
-      x = adam_root<BITS8>(x); y = adam_root<BITS8>(y);
-      root[i] = pack2(x, y);
-      unpack2(fma2(root[i], both2(rc2), both2(a.eps)), d, e);
-      unpack2(mul2(m[i], both2(lr1)), x, y);
-      w[2 * i] = fmaf(__uint_as_float(r.w[2 * i]), keep, -__fdividef(x, d));
-      w[2 * i + 1] = fmaf(__uint_as_float(r.w[2 * i + 1]), keep, -__fdividef(y, e));
-    }
-    if (o.words()) {
-      store_words(o.master, reinterpret_cast<const uint32_t (&)[8]>(w));
-      if (o.p) *reinterpret_cast<bf16x8*>(o.p) = pack8(w);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; e++) if (e < o.left) {
-        o.master[e] = w[e];
-        if (o.p) o.p[e] = __float2bfloat16_rn(w[e]);
-      }
-    }
-    const long long s = block * 128 + l16 * 8;
-    if (BITS8) {
-      uint32_t random[8], bm, bv;
-#pragma unroll
-      for (int e = 0; e < 8; e++) random[e] = random_bits((uint32_t)s + e, key);
-      if (o.left < 8) {                                     // what lies beyond the tensor stays zero
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-          float x, y;
-          unpack2(m[i], x, y); m[i] = pack2(2 * i < o.left ? x : 0.f, 2 * i + 1 < o.left ? y : 0.f);
-          unpack2(root[i], x, y); root[i] = pack2(2 * i < o.left ? x : 0.f, 2 * i + 1 < o.left ? y : 0.f);
-          unpack2(v[i], x, y); v[i] = pack2(2 * i < o.left ? x : 0.f, 2 * i + 1 < o.left ? y : 0.f);
-        }
-      }
-      *reinterpret_cast<uint2*>(static_cast<uint8_t*>(a.m) + s) = round_block<false>(m, m, random, mask, bm);
-      *reinterpret_cast<uint2*>(static_cast<uint8_t*>(a.v) + s) = round_block<true>(root, v, random, mask, bv);
-      if (l16 == 0) { a.ms[block] = bm; a.vs[block] = bv; }
-    } else {
-      store_words(static_cast<float*>(a.m) + s, reinterpret_cast<const uint32_t (&)[8]>(m));
-      store_words(static_cast<float*>(a.v) + s, reinterpret_cast<const uint32_t (&)[8]>(v));
-    }
+  for (long long block = blockIdx.x * 8ll + (threadIdx.x >> 5); block < a.blocks; block += stride) {
+    if (block >= now.end) adam_find(a, block, now);
+    const long long i = (block - now.first) * 128 + l * E, s = block * 128 + l * E;
+    const int left = (int)min((long long)E, now.n - i);    // elements of this lane (not positive: none)
+    const bool words = (now.flags & ADAM_WORDS) && left == E;
+    uint32_t gw[E], w[E];
+    f32x2 m[2], v[2], root[2];
+    load_words(static_cast<const float*>(a.m) + s, reinterpret_cast<uint32_t (&)[E]>(m));
+    load_words(static_cast<const float*>(a.v) + s, reinterpret_cast<uint32_t (&)[E]>(v));
+    if (words) {
+      load_words(now.master + i, w);
+      if (now.flags & ADAM_G_F32) load_words(gradients(now, i), gw); else load_words(gradients(now, i), reinterpret_cast<uint32_t (&)[E / 2]>(gw));
+    } else load_some(gradients(now, i), now.master + i, left, now.flags, gw, w);
+    step.update<false>(a, now.flags, gw, w, m, v, root);
+    store_weights(now.master + i, now.p ? now.p + i : nullptr, left, words, w);
+    store_words(static_cast<float*>(a.m) + s, reinterpret_cast<const uint32_t (&)[E]>(m));
+    store_words(static_cast<float*>(a.v) + s, reinterpret_cast<const uint32_t (&)[E]>(v));
   }
-  __syncthreads();                                        // every thread has read *step
-  if (threadIdx.x == 0 && atomicAdd(a.ticket, 1u) == gridDim.x - 1) { *a.ticket = 0; atomicAdd(a.step, 1); }
+  AdamStep::done(a);
+}
+
+// Moments in 8 bits: a lane has eight elements, sixteen lanes a block, a warp two blocks.  16 bytes an element.
+__global__ void __launch_bounds__(256, 3) adamw_many8_kernel(const AdamArgs a) {
+  constexpr int E = 8;
+  pdl_begin();
+  const AdamStep step(a);
+  const int l = threadIdx.x & 15, second = threadIdx.x >> 4 & 1;
+  const long long stride = gridDim.x * 16ll;
+  AdamNow now;
+  now.at = 0; now.end = -1;
+  for (long long block = blockIdx.x * 16ll + (threadIdx.x >> 4); block - second < a.blocks; block += stride) {
+    const bool there = block < a.blocks;                    // the first half of a warp may have the last block
+    if (there && block >= now.end) adam_find(a, block, now);
+    const long long i = (block - now.first) * 128 + l * E, s = block * 128 + l * E;
+    const int left = there ? (int)min((long long)E, now.n - i) : 0;
+    const bool words = (now.flags & ADAM_WORDS) && left == E;
+    uint32_t gw[E], w[E], mw[2] = {0, 0}, vw[2] = {0, 0}, mb = 0, vb = 0;
+    if (there) {
+      load_words(static_cast<const uint8_t*>(a.m) + s, mw);
+      load_words(static_cast<const uint8_t*>(a.v) + s, vw);
+      mb = a.ms[block]; vb = a.vs[block];
+    }
+    if (words) {
+      load_words(now.master + i, w);
+      if (now.flags & ADAM_G_F32) load_words(gradients(now, i), gw); else load_words(gradients(now, i), reinterpret_cast<uint32_t (&)[E / 2]>(gw));
+    } else load_some(gradients(now, i), now.master + i, left, now.flags, gw, w);
+    f32x2 m[4], v[4], root[4];
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+      e4m3_values(mw[k], scale_value(mb), reinterpret_cast<f32x2 (&)[2]>(m[2 * k]));
+      e4m3_values(vw[k], scale_value(vb), reinterpret_cast<f32x2 (&)[2]>(v[2 * k]));
+    }
+#pragma unroll
+    for (int k = 0; k < 4; k++) v[k] = mul2(v[k], v[k]);
+    step.update<true>(a, now.flags, gw, w, m, v, root);
+    store_weights(now.master + i, now.p ? now.p + i : nullptr, left, words, w);
+    uint32_t random[E];
+#pragma unroll
+    for (int e = 0; e < E; e++) random[e] = random_bits((uint32_t)s + e, step.key);
+    if (left < E) {                                         // what lies beyond the tensor stays zero
+#pragma unroll
+      for (int k = 0; k < 4; k++)
+        for (f32x2* z : {&m[k], &root[k], &v[k]}) {
+          float x, y; unpack2(*z, x, y);
+          *z = pack2(2 * k < left ? x : 0.f, 2 * k + 1 < left ? y : 0.f);
+        }
+    }
+    uint2 om, ov;
+    round_moments(m, v, root, random, om, ov, mb, vb);
+    if (!there) continue;
+    *reinterpret_cast<uint2*>(static_cast<uint8_t*>(a.m) + s) = om;
+    *reinterpret_cast<uint2*>(static_cast<uint8_t*>(a.v) + s) = ov;
+    if (l == 0) { a.ms[block] = mb; a.vs[block] = vb; }
+  }
+  AdamStep::done(a);
 }
 
 }  // namespace piccl_ops
@@ -275,9 +307,9 @@ int piccl_ops_adamw_many(const void* tensors, int count, long long blocks, int b
   if ((reinterpret_cast<uintptr_t>(m) | reinterpret_cast<uintptr_t>(v)) & 15) return -2;
   AdamArgs a{static_cast<const AdamTensor*>(tensors), count, blocks, m, v, (uint8_t*)ms, (uint8_t*)vs, lr, (float)b1, (float)(1 - b1), (float)b2, (float)(1 - b2), eps, wd, log(b1), log(b2),
              gscale, gscale_dev, step, ticket, seed};
-  const long long want = (blocks + 15) / 16, most = 148 * (bits8 ? 3 : 2);
-  const unsigned grid = (unsigned)(want < 1 ? 1 : want < most ? want : most);
-  const cudaError_t e = launch_pdl(bits8 ? adamw_many_kernel<true> : adamw_many_kernel<false>, dim3(grid), 256, 0, (cudaStream_t)stream, a);
+  const long long want = bits8 ? (blocks + 15) / 16 : (blocks + 7) / 8, most = 148 * (bits8 ? 3 : 5);
+  const dim3 grid((unsigned)(want < 1 ? 1 : want < most ? want : most));
+  const cudaError_t e = launch_pdl(bits8 ? adamw_many8_kernel : adamw_many_kernel, grid, 256, 0, (cudaStream_t)stream, a);
   return e == cudaSuccess ? 0 : (int)e;
 }
 
