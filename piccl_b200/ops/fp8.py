@@ -29,7 +29,7 @@ from .gemm_sm100 import _native, _ptr
 E4M3 = torch.float8_e4m3fn
 _QUANTIZE = [C.c_void_p, C.c_int] + [C.c_longlong] * 3 + [C.c_void_p] * 4 + [C.c_int, C.c_void_p]
 _GEMM = [C.c_void_p] * 6 + [C.c_int] * 3 + [C.c_longlong, C.c_int, C.c_void_p]
-_SCRATCH = [C.c_void_p, C.c_int, C.c_longlong, C.c_int, C.c_longlong, C.c_int]
+_SCRATCH = [C.c_void_p, C.c_int, C.c_longlong, C.c_int, C.c_int, C.c_longlong, C.c_int]
 _LINEAR = [C.c_void_p, C.c_int, C.c_longlong] + [C.c_void_p] * 4 + [C.c_int] + [C.c_void_p] * 4 + [C.c_int] * 2 + [C.c_longlong, C.c_void_p]
 _fast = None
 
@@ -162,7 +162,7 @@ def linear(x: torch.Tensor, w: Fp8, out: torch.Tensor, bias: Optional[torch.Tens
     M, K = x.shape
     if w.values.dim() != 2 or w.values.shape[1] != (K + 127) // 128 * 128:
         raise ValueError(f"linear: weights of {K} columns wanted, got {tuple(w.values.shape)}")
-    if keep is None and M and K and M <= 64 and not _native("piccl_ops_fp8_linear_scratch", _SCRATCH)(x.data_ptr(), x.dtype == torch.float32, x.stride(0) if M > 1 else K, M, K, False):
+    if keep is None and M and K and M <= 64 and not _native("piccl_ops_fp8_linear_scratch", _SCRATCH)(x.data_ptr(), x.dtype == torch.float32, x.stride(0) if M > 1 else K, M, w.values.shape[0], K, False):
         _check_product((M, w.values.shape[1]), w, out, bias)
         if out.device != x.device:
             raise ValueError("linear: tensors of one CUDA device wanted")

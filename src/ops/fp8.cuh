@@ -11,7 +11,8 @@
 namespace piccl_ops {
 
 // fp8_few.cu: products of at most 64 rows
-int fp8_few(const bf16* x, long long stride, const void* a, const void* sa, const void* b, const void* sb, const void* bias, void* out, int f32, int M, int N, int K, int splits, void* stream);
+bool fp8_few_takes(int M, int N, long long K);
+int fp8_few(const bf16* x, long long stride, const void* a, const void* sa, const void* b, const void* sb, const void* bias, void* out, int f32, int M, int N, int K, void* stream);
 
 // bits of |x|, 0 for what is not finite
 __device__ __forceinline__ uint32_t finite_bits(float x) { const uint32_t u = __float_as_uint(x) & 0x7fffffffu; return u < 0x7f800000u ? u : 0u; }

@@ -1,243 +1,213 @@
 // The products of fp8_gemm.cu for at most 64 rows, as in decoding: C[M, N] = A[M, K] B[N, K]^T + bias, bound by the bytes of B.
 //
-// The operands change places: a CTA has 128 rows of B as the rows of its tile and all M rows of A as its columns (16, 32 or 64), so no part of the instruction works on rows that are not
-// there.  K is split over the CTAs of a cluster until the chip has a CTA or two per SM; each leaves its partial sums in shared memory, and every CTA adds a share of them up, in the order
-// of the ranks, through distributed shared memory.  A may come as bf16: eight warps round it on its way into shared memory (a block of 128 each), which saves the launch, and the
-// scratch, of a quantiser.
-#include <cstring>
-#include <mutex>
-#include "../include/sm100_gemm_pair.cuh"
+// A block has 16 or 32 rows of B, its eight warps take the k-blocks of 128 in turn: a warp reads its part of B straight into the fragments of mma.sync (B's rows are the fragment's 16 rows, A's
+// rows its 8 columns; k may stand in any order that both sides share, so a lane's 16 bytes are contiguous), sums a block of 128 and adds it to its sums in fp32, scaled by the two powers of two.  The
+// warps' sums meet in shared memory and are added in the warps' order.  No part of B is staged and nothing waits for another block; a warp has several blocks of B under way while all warps
+// bring A into shared memory.  (Tensor cores that need descriptors, TMEM and barriers have nothing to gain where 2 KiB a warp and block are read once.)
+// A may come as bf16: it is rounded on its way into shared memory, which saves the launch, and the scratch, of a quantiser; every block reads all of A for it.
+#include <atomic>
 #include "fp8.cuh"
-#include "fp8_mma.cuh"
 
 namespace piccl_ops {
 
-using namespace sm100;
-
 struct FewArgs {
-  CUtensorMap tw, sw, tx, sx;        // B's values and scales, A's
+  const uint8_t *w, *sw, *a, *sa;    // B's values and scales, A's
   const bf16* x; long long stride;   // or A itself
   const bf16* bias; void* out;
-  int M, N, K, kb, k4, splits;
-  int* status;
-};
-constexpr int FEW_THREADS = 320;
-
-template <int T>
-struct FewSmem {
-  static constexpr int STAGES = T <= 32 ? 5 : 4, W_BYTES = 128 * 128, X_BYTES = T * 128, STAGE = W_BYTES + X_BYTES;
-  static constexpr int SF_OFF = STAGES * STAGE, BAR_OFF = SF_OFF + STAGES * 1024, TOTAL = BAR_OFF + (2 * STAGES + 1) * 8 + 8, DYNAMIC = TOTAL + 1024;
-  static_assert(128 * T * 4 <= STAGES * STAGE && 2 * (DYNAMIC + 2048) <= 228 * 1024, "partial sums lie over the ring; two CTAs to an SM");
+  int M, N, K, kb, k4;
 };
 
-__device__ __forceinline__ float cluster_load(const float* p, uint32_t rank) {
-  uint32_t a; float v;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
-  return v;
+__device__ __forceinline__ void mma_e4m3(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-template <int T, bool QUANT, typename O>
-__global__ void __launch_bounds__(FEW_THREADS) fp8_few_kernel(const __grid_constant__ FewArgs a) {
-  typedef FewSmem<T> L;
-  constexpr int STAGES = L::STAGES;
-  constexpr uint32_t COLS = T == 16 ? 32 : T == 32 ? 64 : 128;
-  extern __shared__ __align__(1024) uint8_t smem_raw[];
-  __shared__ int s_abort;
-  __shared__ uint32_t s_tmem;
-  uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint64_t* const full = reinterpret_cast<uint64_t*>(smem + L::BAR_OFF);
-  uint64_t *const empty = full + STAGES, *const done = empty + STAGES;
-  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-  const int rank = blockIdx.x % a.splits, tile = blockIdx.x / a.splits, kb0 = (int)((long long)a.kb * rank / a.splits), kb1 = (int)((long long)a.kb * (rank + 1) / a.splits);
-  if (threadIdx.x == 0) {
-    s_abort = 0;
-    for (int s = 0; s < STAGES; s++) { mbar_init(&full[s], QUANT ? 2 : 1); mbar_init(&empty[s], 1); }
-    mbar_init(done, 1);
-    fence_barrier_init();
-  }
-  if (warp == 1) tmem_alloc_cta(&s_tmem, COLS);
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem = s_tmem;
-  pdl_begin();
-  bool ok = true;
+// A in shared memory: 8 T rows of kb * 128 bytes, 16-byte pieces of a block moved by the row so that eight lanes beside each other, four pieces of two rows, meet in no bank, and the scales as
+// powers of two in fp32 for each block and row.
+struct FewA {
+  uint4* x; float* f; int kb;
+  __device__ __forceinline__ uint4* piece(int row, int block, int i) const { return x + ((size_t)row * kb + block) * 8 + (i ^ (row & 1) << 2 ^ (row >> 1 & 3)); }
+  __device__ __forceinline__ float* power(int row, int block, int rows) const { return f + (size_t)block * rows + row; }
+};
 
-  if (warp == 0) {
-    const bool issuer = elect_one();
-    for (int kb = kb0; kb < kb1; kb++) {
-      const int j = kb - kb0, st = j % STAGES;
-      if (!mbar_wait(&empty[st], ((j / STAGES) & 1) ^ 1, &s_abort, kPairWaitLimitNs)) { ok = false; break; }
-      uint8_t *const pw = smem + st * L::STAGE, *const ps = smem + L::SF_OFF + st * 1024;
-      if (issuer) {
-        const bool scales = kb == kb0 || (kb & 3) == 0;
-        mbar_arrive_expect_tx(&full[st], L::W_BYTES + (QUANT ? 0 : L::X_BYTES) + (scales ? (QUANT ? 512 : 1024) : 0));
-        tma_load_2d(pw, &a.tw, kb * 128, tile * 128, &full[st]);
-        if (!QUANT) tma_load_2d(pw + L::W_BYTES, &a.tx, kb * 128, 0, &full[st]);
-        if (scales) {
-          tma_load_2d(ps, &a.sw, 0, tile * a.k4 + (kb >> 2), &full[st]);
-          if (!QUANT) tma_load_2d(ps + 512, &a.sx, 0, kb >> 2, &full[st]);
+// R: groups of 16 rows of B, T: groups of 8 rows of A, D: blocks of B that a warp has under way
+template <int R, int T, int D, bool QUANT, typename O>
+__global__ void __launch_bounds__(256, R * T <= 2 ? 2 : 1) fp8_few_kernel(const FewArgs a) {
+  constexpr int ROWS = 16 * R, COLS = 8 * T;
+  extern __shared__ __align__(16) uint4 few_smem[];
+  const FewA A{few_smem, reinterpret_cast<float*>(few_smem + (size_t)COLS * a.kb * 8), a.kb};
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int row0 = blockIdx.x * ROWS;
+  const long long pitch = 128ll * a.kb;
+  // B on its way into L2 while the kernel before this one ends (a hint: whatever that kernel writes is seen all the same)
+  for (int i = threadIdx.x; i < ROWS * a.kb; i += 256) {
+    const int row = row0 + i / a.kb;
+    if (row < a.N) asm volatile("prefetch.global.L2 [%0];" ::"l"(a.w + row * pitch + (i % a.kb) * 128ll));
+  }
+  pdl_begin();
+  struct Part { uint4 w[R][2][2]; uint32_t s[R][2]; } part[D];      // rows g and g + 8 of a group, 16 bytes of each of two chunks of 64 k; their scales
+  auto load = [&](Part& p, int kb) {
+#pragma unroll
+    for (int r = 0; r < R; r++)
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        const int row = row0 + 16 * r + 8 * h + g;
+#pragma unroll
+        for (int c = 0; c < 2; c++) p.w[r][h][c] = row < a.N ? __ldg(reinterpret_cast<const uint4*>(a.w + row * pitch + kb * 128ll + c * 64 + t * 16)) : make_uint4(0, 0, 0, 0);
+        p.s[r][h] = row < a.N ? a.sw[scale_at(row, kb, a.k4)] : 1u;
+      }
+  };
+#pragma unroll
+  for (int d = 0; d < D; d++) if (warp + 8 * d < a.kb) load(part[d], warp + 8 * d);
+  // A: 8 lanes to a row and block, 16 values each, U of them on their way at a time.  (Rows from M on stay what they were: they only reach sums that nobody reads.)
+  {
+    constexpr int U = QUANT ? 4 : 8;
+    const int l8 = threadIdx.x & 7, items = a.M * a.kb, all = (items + 31) / 32 * 32;      // whole warps go round together
+    for (int i0 = threadIdx.x >> 3; i0 < all; i0 += 32 * U) {
+      uint32_t w[U][QUANT ? 8 : 4];
+#pragma unroll
+      for (int u = 0; u < U; u++) {
+        const int i = i0 + 32 * u, m = i / a.kb, kb = i - m * a.kb, c = kb * 128 + l8 * 16;
+#pragma unroll
+        for (int e = 0; e < (QUANT ? 8 : 4); e++) w[u][e] = 0;
+        if constexpr (QUANT) {
+#pragma unroll
+          for (int h = 0; h < 2; h++) if (i < items && c + 8 * h < a.K) {
+            const uint4 v = __ldg(reinterpret_cast<const uint4*>(a.x + m * a.stride + c + 8 * h));
+            w[u][4 * h] = v.x; w[u][4 * h + 1] = v.y; w[u][4 * h + 2] = v.z; w[u][4 * h + 3] = v.w;
+          }
+        } else if (i < items) {
+          const uint4 v = __ldg(reinterpret_cast<const uint4*>(a.a + m * pitch + c));
+          w[u][0] = v.x; w[u][1] = v.y; w[u][2] = v.z; w[u][3] = v.w;
         }
       }
-      __syncwarp();
-    }
-  } else if (warp == 1) {
-    const bool issuer = elect_one();
-    constexpr uint32_t idesc = make_idesc_mxf8(128, T);
-    const uint64_t dw0 = make_smem_desc_k128(smem), dx0 = make_smem_desc_k128(smem + L::W_BYTES), ds0 = make_smem_desc_scales(smem + L::SF_OFF);
-    for (int kb = kb0; kb < kb1; kb++) {
-      const int j = kb - kb0, st = j % STAGES;
-      if (!mbar_wait(&full[st], (j / STAGES) & 1, &s_abort, kPairWaitLimitNs)) { ok = false; break; }
-      tc_fence_after();
-      const uint64_t dw = desc_advance(dw0, st * L::STAGE), dx = desc_advance(dx0, st * L::STAGE), ds = desc_advance(ds0, st * 1024);
-      if (issuer) {
-        const bool scales = kb == kb0 || (kb & 3) == 0;
-        if (scales) scales_to_tmem(tmem + T, ds);
-        if (QUANT || scales) scales_to_tmem(tmem + T + 4, desc_advance(ds, 512));
-        const uint32_t byte = kb & 3;
 #pragma unroll
-        for (int k = 0; k < 4; k++) umma_mxf8(tmem, desc_advance(dw, k * 32), desc_advance(dx, k * 32), idesc | idesc_bytes(byte, QUANT ? 0 : byte), tmem + T, tmem + T + 4, j != 0 || k != 0);
-        umma_commit_cta(&empty[st]);
-      }
-      __syncwarp();
-    }
-    if (ok && issuer) umma_commit_cta(done);
-    __syncwarp();
-  } else if (QUANT) {
-    // a warp has every eighth block of the slice: 8 lanes to a row, 16 values each
-    const int sub = lane >> 3, l8 = lane & 7;
-    for (int kb = kb0 + warp - 2; kb < kb1 && ok; kb += 8) {
-      const int j = kb - kb0, st = j % STAGES;
-      uint8_t *const px = smem + st * L::STAGE + L::W_BYTES, *const ps = smem + L::SF_OFF + st * 1024 + 512;
-      const int c = kb * 128 + l8 * 16;
-      bool waited = false;
-#pragma unroll 1
-      for (int r0 = 0; r0 < T && r0 < a.M; r0 += 16) {
-        Eight<bf16> v[4][2];
+      for (int u = 0; u < U; u++) {
+        const int i = i0 + 32 * u, m = i / a.kb, kb = i - m * a.kb;
+        if (i - (threadIdx.x >> 3 & 3) >= items) break;      // none of the warp's four
+        uint4 piece; uint32_t byte = 1;
+        if constexpr (QUANT) {
+          Eight<bf16> v[2];
 #pragma unroll
-        for (int i = 0; i < 4; i++)
-#pragma unroll
-          for (int h = 0; h < 2; h++) {
-#pragma unroll
-            for (int e = 0; e < 4; e++) v[i][h].w[e] = 0;
-            if (r0 + 4 * i + sub < a.M && c + 8 * h < a.K) v[i][h].load(a.x + (r0 + 4 * i + sub) * a.stride + c + 8 * h);
-          }
-        if (!waited) { ok = mbar_wait(&empty[st], ((j / STAGES) & 1) ^ 1, &s_abort, kPairWaitLimitNs); waited = true; if (!ok) break; }
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-          const int r = r0 + 4 * i + sub;
-          uint32_t top = max(top8(v[i][0]), top8(v[i][1]));
+          for (int e = 0; e < 4; e++) { v[0].w[e] = w[u][e]; v[1].w[e] = w[u][4 + e]; }
+          uint32_t top = max(top8(v[0]), top8(v[1]));
           const bool odd = __any_sync(0xffffffffu, top >= kInf);
-          if (odd) top = max(finite_top8(v[i][0]), finite_top8(v[i][1]));
+          if (odd) top = max(finite_top8(v[0]), finite_top8(v[1]));
 #pragma unroll
           for (int o = 4; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-          const uint32_t byte = scale_byte(top);
+          byte = scale_byte(top);
           const float f = scale_inverse(byte);
-          const uint2 lo = pack_row(v[i][0], f, odd), hi = pack_row(v[i][1], f, odd);
-          if (r < a.M) {
-            *reinterpret_cast<uint4*>(px + r * 128 + ((l8 ^ (r & 7)) << 4)) = make_uint4(lo.x, lo.y, hi.x, hi.y);
-            if (l8 == 0) *reinterpret_cast<uint32_t*>(ps + (r & 31) * 16 + (r >> 5) * 4) = byte;
-          }
+          const uint2 lo = pack_row(v[0], f, odd), hi = pack_row(v[1], f, odd);
+          piece = make_uint4(lo.x, lo.y, hi.x, hi.y);
+        } else {
+          piece = make_uint4(w[u][0], w[u][1], w[u][2], w[u][3]);
+          if (l8 == 0 && i < items) byte = a.sa[scale_at(m, kb, a.k4)];
+        }
+        if (i < items) {
+          *A.piece(m, kb, l8) = piece;
+          if (l8 == 0) *A.power(m, kb, COLS) = scale_value(byte);
         }
       }
-      fence_proxy_async();
-      __syncwarp();
-      if (ok && lane == 0) mbar_arrive(&full[st]);
     }
   }
-  // partial sums, over the ring: all of it has been read
-  float* const part = reinterpret_cast<float*>(smem);
-  if (warp >= 2 && warp < 6 && ok) {
-    ok = mbar_wait(done, 0, &s_abort, kPairWaitLimitNs);
-    tc_fence_after();
-    if (ok) {
-      const int quarter = warp & 3;
+  __syncthreads();
+  float acc[R][T][4];
 #pragma unroll
-      for (int q = 0; q < T / 16; q++) {
-        uint32_t r[16];
-        tmem_ld_32x16(tmem + ((uint32_t)(quarter * 32) << 16) + 16 * q, r);
-        tmem_ld_wait();
+  for (int r = 0; r < R; r++)
 #pragma unroll
-        for (int i = 0; i < 16; i++) if (16 * q + i < a.M) part[(16 * q + i) * 128 + quarter * 32 + lane] = __uint_as_float(r[i]);
+    for (int n = 0; n < T; n++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) acc[r][n][i] = 0.f;
+  for (int base = warp; base < a.kb; base += 8 * D) {
+#pragma unroll
+    for (int d = 0; d < D; d++) {
+      const int kb = base + 8 * d;
+      if (kb >= a.kb) break;
+      const Part& p = part[d];
+#pragma unroll
+      for (int n = 0; n < T; n++) {
+        uint4 b[2];                                        // row 8 n + g of A
+#pragma unroll
+        for (int k = 0; k < 2; k++) b[k] = *A.piece(8 * n + g, kb, 4 * k + t);
+        const float2 fx = *reinterpret_cast<const float2*>(A.power(8 * n + 2 * t, kb, COLS));
+#pragma unroll
+        for (int r = 0; r < R; r++) {
+          float c[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int k = 0; k < 2; k++) {
+            mma_e4m3(c, p.w[r][0][k].x, p.w[r][1][k].x, p.w[r][0][k].y, p.w[r][1][k].y, b[k].x, b[k].y);
+            mma_e4m3(c, p.w[r][0][k].z, p.w[r][1][k].z, p.w[r][0][k].w, p.w[r][1][k].w, b[k].z, b[k].w);
+          }
+          const float f0 = scale_value(p.s[r][0]), f1 = scale_value(p.s[r][1]);
+          acc[r][n][0] = fmaf(c[0] * f0, fx.x, acc[r][n][0]); acc[r][n][1] = fmaf(c[1] * f0, fx.y, acc[r][n][1]);
+          acc[r][n][2] = fmaf(c[2] * f1, fx.x, acc[r][n][2]); acc[r][n][3] = fmaf(c[3] * f1, fx.y, acc[r][n][3]);
+        }
       }
+      if (kb + 8 * D < a.kb) load(part[d], kb + 8 * D);
     }
   }
-  if (!ok) { *(volatile int*)&s_abort = 1; if (lane == 0) atomicExch(a.status, 20 + warp); }
-  tc_fence_before();
-  __syncwarp();
-  cluster_sync_all();
-  const int total = a.M * 128, share = (total + a.splits - 1) / a.splits, end = min(total, share * (rank + 1));
-  for (int e = share * rank + threadIdx.x; e < end; e += FEW_THREADS) {
-    const int n = tile * 128 + (e & 127);
+  __syncthreads();                                         // A has been read: the sums take its place
+  float* const sums = reinterpret_cast<float*>(few_smem);  // [8][COLS][ROWS + 1]
+#pragma unroll
+  for (int r = 0; r < R; r++)
+#pragma unroll
+    for (int n = 0; n < T; n++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) sums[(warp * COLS + 8 * n + 2 * t + (i & 1)) * (ROWS + 1) + 16 * r + 8 * (i >> 1) + g] = acc[r][n][i];
+  __syncthreads();
+  for (int e = threadIdx.x; e < a.M * ROWS; e += 256) {
+    const int m = e / ROWS, n = e % ROWS;
+    if (row0 + n >= a.N) continue;
     float s = 0.f;
-    for (int p = 0; p < a.splits; p += 4) {
-      float v[4];
 #pragma unroll
-      for (int q = 0; q < 4; q++) v[q] = p + q < a.splits ? cluster_load(part + e, p + q) : 0.f;
-#pragma unroll
-      for (int q = 0; q < 4; q++) s += v[q];
-    }
-    if (n < a.N) {
-      if (a.bias) s += __bfloat162float(a.bias[n]);
-      static_cast<O*>(a.out)[(size_t)(e >> 7) * a.N + n] = (O)s;
-    }
+    for (int q = 0; q < 8; q++) s += sums[(q * COLS + m) * (ROWS + 1) + n];
+    if (a.bias) s += __bfloat162float(a.bias[row0 + n]);
+    static_cast<O*>(a.out)[(size_t)m * a.N + row0 + n] = (O)s;
   }
-  cluster_sync_all();                                      // nobody leaves while its sums are being read
-  if (*(volatile int*)&s_abort) {                          // copies in flight get time to land
-    const unsigned long long t0 = gtime_ns();
-    while (gtime_ns() - t0 < 2000000ull) __nanosleep(1000);
-    __syncthreads();
-  }
-  if (warp == 1) { tc_fence_after(); tmem_dealloc_cta(tmem, COLS); }
 }
 
-// ------------------------------------------------------------------ host
-typedef void (*FewFn)(FewArgs);
-struct FewVariant { int t, quant, f32; FewFn fn; int smem; };
-#define V_(T, Q, F, O) {T, Q, F, fp8_few_kernel<T, Q != 0, O>, FewSmem<T>::DYNAMIC}
-static const FewVariant g_few[] = {V_(16, 0, 0, bf16), V_(32, 0, 0, bf16), V_(64, 0, 0, bf16), V_(16, 0, 1, float), V_(32, 0, 1, float), V_(64, 0, 1, float),
-                                   V_(16, 1, 0, bf16), V_(32, 1, 0, bf16), V_(64, 1, 0, bf16), V_(16, 1, 1, float), V_(32, 1, 1, float), V_(64, 1, 1, float)};
-#undef V_
-
-static int few_ready(int dev) {
-  static std::mutex mu;
-  static bool ready[64] = {false};
-  std::lock_guard<std::mutex> l(mu);
-  if (ready[dev]) return 0;
-  for (const FewVariant& v : g_few) if (cudaFuncSetAttribute((const void*)v.fn, cudaFuncAttributeMaxDynamicSharedMemorySize, v.smem) != cudaSuccess) return -4;
-  ready[dev] = true;
-  return 0;
+static size_t few_smem_bytes(int rows, int cols, int kb) {
+  const size_t a = (size_t)cols * kb * (128 + 4), sums = (size_t)8 * cols * (rows + 1) * 4;
+  return a > sums ? a : sums;
 }
+constexpr size_t kFewSmem = 200 * 1024;
 
-// x: A in bf16 (rows on 16-byte boundaries, K a multiple of 8), or null: values a with scales sa
-int fp8_few(const bf16* x, long long stride, const void* a, const void* sa, const void* b, const void* sb, const void* bias, void* out, int f32, int M, int N, int K, int splits, void* stream) {
+template <int R, int T, int D, bool QUANT, typename O> static int few(const FewArgs& g, cudaStream_t s) {
+  static std::atomic<bool> ready[64];
   int dev = 0; cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64) return -6;
-  const int rc = few_ready(dev); if (rc) return rc;
-  const FewVariant* v = nullptr;
-  for (const FewVariant& c : g_few) if (!v && c.t >= M && c.quant == (x != nullptr) && c.f32 == (f32 != 0)) v = &c;
-  if (!v) return -1;
-  FewArgs g;
-  memset(&g, 0, sizeof g);
-  g.x = x; g.stride = stride; g.bias = (const bf16*)bias; g.out = out; g.M = M; g.N = N; g.K = K; g.kb = (K + 127) / 128; g.k4 = (g.kb + 3) / 4;
-  const int tiles = (N + 127) / 128;
-  if (!splits) for (splits = 1; splits < 8 && 2 * splits <= g.kb && tiles * splits * 2 <= 2 * 148; splits *= 2) {}
-  if (splits > g.kb) return -1;
-  g.splits = splits;
-  const uint64_t kp = 128ull * g.kb;
-  if (!fp8_map(&g.tw, 1, b, N, kp, 128, 128, true) || !fp8_map(&g.sw, 4, sb, (uint64_t)tiles * g.k4, 128, 1, 128, false)) return -3;
-  if (x) { g.tx = g.tw; g.sx = g.sw; }
-  else if (!fp8_map(&g.tx, 1, a, M, kp, v->t, 128, true) || !fp8_map(&g.sx, 4, sa, g.k4, 128, 1, 128, false)) return -3;
-  g.status = status_word(STATUS_GEMM);
-  if (!g.status) return -7;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(tiles * splits); cfg.blockDim = dim3(FEW_THREADS); cfg.dynamicSmemBytes = v->smem; cfg.stream = (cudaStream_t)stream;
-  cudaLaunchAttribute at[2];
-  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization; at[0].val.programmaticStreamSerializationAllowed = 1;
-  at[1].id = cudaLaunchAttributeClusterDimension; at[1].val.clusterDim.x = splits; at[1].val.clusterDim.y = 1; at[1].val.clusterDim.z = 1;
-  cfg.attrs = at; cfg.numAttrs = 2;
-  return cudaLaunchKernelEx(&cfg, v->fn, g) == cudaSuccess ? 0 : -5;
+  const auto fn = fp8_few_kernel<R, T, D, QUANT, O>;
+  if (!ready[dev]) {
+    if (cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewSmem) != cudaSuccess) return -4;
+    ready[dev] = true;
+  }
+  return launch_pdl(fn, dim3((g.N + 16 * R - 1) / (16 * R)), 256, few_smem_bytes(16 * R, 8 * T, g.kb), s, g) == cudaSuccess ? 0 : -5;
+}
+template <bool QUANT, typename O> static int few(const FewArgs& g, cudaStream_t s) {
+  const bool wide = g.N > 32 * 148;
+  if (g.M <= 8) return wide ? few<2, 1, 2, QUANT, O>(g, s) : few<1, 1, 4, QUANT, O>(g, s);
+  if (g.M <= 16) return wide ? few<2, 2, 2, QUANT, O>(g, s) : few<1, 2, 3, QUANT, O>(g, s);
+  if (g.M <= 32) return few<1, 4, 3, QUANT, O>(g, s);
+  return few<1, 8, 2, QUANT, O>(g, s);
+}
+
+// Whether the kernel is the one for M rows of K values: A has to fit into shared memory, and what the blocks of an SM take in of it, each for itself, has to be little beside B.  Against the quantiser
+// and the pairs' kernel (us, one launch and two): M 1, N 4096, K 1024 / 4096 / 8192: 3.9 / 6.3 / 9.5 and 7.8 / 16.1 / 28.6; M 8: 4.0 / 9.2 / 15.5 and 6.8 / 13.9 / 24.8; M 16, N 1024, K 2048 / 4096: 5.9 / 10.8
+// and 7.1 / 9.5; M 8, N 16384, K 1024 / 4096: 9.0 / 25.7 and 9.8 / 20.8; M 32, N 1024, K 1024 / 2048: 5.7 / 9.0 and 6.5 / 7.2.
+bool fp8_few_takes(int M, int N, long long K) {
+  if (M > 64 || K > 1 << 20) return false;
+  const int cols = M <= 8 ? 8 : M <= 16 ? 16 : M <= 32 ? 32 : 64, kb = (int)((K + 127) / 128);
+  const bool wide = N > 32 * 148 && M <= 16;
+  const long long blocks = (N + (wide ? 32 : 16) - 1) / (wide ? 32 : 16), taken = (blocks + 147) / 148 * M * kb;
+  return few_smem_bytes(32, cols, kb) <= kFewSmem && taken <= (M > 8 ? 256 : N > 32 * 148 ? 512 : 1024);
+}
+// x: A in bf16 (on 16-byte boundaries, K a multiple of 8), or null: values a with scales sa
+int fp8_few(const bf16* x, long long stride, const void* a, const void* sa, const void* b, const void* sb, const void* bias, void* out, int f32, int M, int N, int K, void* stream) {
+  const FewArgs g{(const uint8_t*)b, (const uint8_t*)sb, (const uint8_t*)a, (const uint8_t*)sa, x, stride, (const bf16*)bias, out, M, N, K, (K + 127) / 128, (K + 511) / 512};
+  const cudaStream_t s = (cudaStream_t)stream;
+  if (!fp8_few_takes(M, N, K)) return -1;
+  if (x) return f32 ? few<true, float>(g, s) : few<true, bf16>(g, s);
+  return f32 ? few<false, float>(g, s) : few<false, bf16>(g, s);
 }
 
 }  // namespace piccl_ops

@@ -26,14 +26,16 @@ struct Fp8Args {
 constexpr int FP8_BM = 128, FP8_BK = 128, FP8_THREADS = 320;
 constexpr uint32_t kScaleCol = 496;        // TMEM columns: accumulators from 0 on, scales of A 4 from here, of B 8
 
-template <int TN, int STAGES>
+// AR: rows of A that are staged.  A product of at most 64 rows stages 64: the MMA reads 128 all the same, and what it finds beyond (the next stage) goes into rows that nobody reads.
+template <int TN, int STAGES, int AR>
 struct Fp8Smem {
-  static constexpr int A_BYTES = FP8_BM * FP8_BK, B_BYTES = TN / 2 * FP8_BK, STAGE = A_BYTES + B_BYTES;
+  static constexpr int A_BYTES = AR * FP8_BK, B_BYTES = TN / 2 * FP8_BK, STAGE = A_BYTES + B_BYTES;
   static constexpr int NSF = TN > 128 ? 3 : 2, SF_BYTES = 512 * NSF;      // atoms of A's rows and of B's columns
-  static constexpr int SF_OFF = STAGES * STAGE, STAGING_OFF = (SF_OFF + STAGES * SF_BYTES + 1023) / 1024 * 1024;
+  static constexpr int B_OFF = STAGES * A_BYTES, SF_OFF = STAGES * STAGE, STAGING_OFF = (SF_OFF + STAGES * SF_BYTES + 1023) / 1024 * 1024;
   static constexpr int BAR_OFF = STAGING_OFF + PAIR_EPI_WARPS * PAIR_STAGING;
   static constexpr int TOTAL = BAR_OFF + (2 * STAGES + 4) * 8 + 16, DYNAMIC = TOTAL + 1024;
   static_assert(DYNAMIC <= 232448, "more shared memory than a CTA can have");
+  static_assert(STAGES * B_BYTES >= FP8_BM * FP8_BK - A_BYTES, "what is read beyond the last stage of A is there");
 };
 
 // 128 bytes of a row of the result
@@ -100,11 +102,11 @@ constexpr int kUnit = 8;           // k-blocks (tiles of 128 columns at most: 64
 
 // TMEM has 512 columns: two accumulators of 256 and the scales do not fit.  They overlap in 16 columns: the MMAs of the next unit wait until the epilogue has those in registers (its warps
 // take the piece with them first), and not for the rest of the tile.
-template <int TN, int STAGES, typename O>
+template <int TN, int STAGES, int AR, typename O>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FP8_THREADS, 1) fp8_pair_kernel(const __grid_constant__ Fp8Args a) {
-  typedef Fp8Smem<TN, STAGES> L;
+  typedef Fp8Smem<TN, STAGES, AR> L;
   constexpr bool OVERLAP = TN > 240, ADD = sizeof(O) == 4;
-  static_assert(!(OVERLAP && ADD), "128 sums a thread do not fit");
+  static_assert(!(OVERLAP && ADD) && TN >= 64, "128 sums a thread do not fit; scales lie at even columns");
   constexpr uint32_t ACC = OVERLAP ? 240 : TN;            // columns between the accumulators
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   __shared__ int s_abort;
@@ -141,7 +143,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FP8_THREADS, 1) fp8_
       bool ok = true;
       for (int kb = 0; kb < a.kb; kb++) {
         if (!mbar_wait(&empty[stage], phase ^ 1, &s_abort, kPairWaitLimitNs)) { if (issuer) atomicExch(a.status, 11); ok = false; break; }
-        uint8_t *const pa = smem + stage * L::STAGE, *const pb = pa + L::A_BYTES, *const ps = smem + L::SF_OFF + stage * L::SF_BYTES;
+        uint8_t *const pa = smem + stage * L::A_BYTES, *const pb = smem + L::B_OFF + stage * L::B_BYTES, *const ps = smem + L::SF_OFF + stage * L::SF_BYTES;
         if (issuer) {
           const bool scales = (kb & 3) == 0;
           if (v == 0) mbar_arrive_expect_tx(&full[stage], 2 * (L::STAGE + (scales ? L::SF_BYTES : 0)));
@@ -163,13 +165,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FP8_THREADS, 1) fp8_
     if (v == 0) {
       const bool issuer = elect_one();
       constexpr uint32_t idesc = make_idesc_mxf8(256, TN);
-      const uint64_t da0 = make_smem_desc_k128(smem), db0 = make_smem_desc_k128(smem + L::A_BYTES), ds0 = make_smem_desc_scales(smem + L::SF_OFF);
+      const uint64_t da0 = make_smem_desc_k128(smem), db0 = make_smem_desc_k128(smem + L::B_OFF), ds0 = make_smem_desc_scales(smem + L::SF_OFF);
       const uint32_t sfa = tmem + kScaleCol, sfb = sfa + 4;
       int stage = 0; uint32_t phase = 0; int local = 0;
       bool ok = true;
       for (int t = first; ok && t < num_tiles && !*(volatile int*)&s_abort; t += stride) {
         int m_blk, n_blk; tile(t, m_blk, n_blk);
-        const uint32_t sfb_t = sfb + (TN == 64 ? 2 * (n_blk & 1) : 0);
+        const uint32_t sfb_t = sfb + (TN == 64 ? 2 * (n_blk & 1) : 0);      // where in its 128 columns the tile begins (an even column of TMEM: tiles of 32 cannot be)
         for (int u = 0; ok && u < units; u++, local++) {
           const int acc = local & 1;
           // overlapping: the edge of the unit before is in registers, and with it all of the one before that; else: this accumulator's unit is
@@ -183,7 +185,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FP8_THREADS, 1) fp8_
           for (int kb = kb0; kb < kb1; kb++) {
             if (!mbar_wait(&full[stage], phase, &s_abort, kPairWaitLimitNs)) { if (issuer) atomicExch(a.status, 13); ok = false; break; }
             tc_fence_after();
-            const uint64_t da = desc_advance(da0, stage * L::STAGE), db = desc_advance(db0, stage * L::STAGE);
+            const uint64_t da = desc_advance(da0, stage * L::A_BYTES), db = desc_advance(db0, stage * L::B_BYTES);
             if (issuer) {
               if ((kb & 3) == 0) {
                 const uint64_t ds = desc_advance(ds0, stage * L::SF_BYTES);
@@ -239,6 +241,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FP8_THREADS, 1) fp8_
           fence_proxy_async();
           __syncwarp();
           if (lane == 0) { tma_store_2d(&a.tc, staging, col, row0); bulk_commit(); }
+          __syncwarp();
         } else {
           __syncwarp();
           store_rows(staging, static_cast<O*>(a.out) + (size_t)row0 * a.N + col, a.N, a.M - row0, a.N - col, lane);
@@ -251,9 +254,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FP8_THREADS, 1) fp8_
         if (!mbar_wait(&tmem_full[local & 1], (local >> 1) & 1, &s_abort, kPairWaitLimitNs)) { atomicExch(a.status, 14); return false; }
         tc_fence_after();
         if (OVERLAP && !edge && lane == 0) mbar_arrive_leader(&tmem_empty[0]);
+        __syncwarp();                                      // tcgen05.ld, which comes next, wants the whole warp at one place: so after everything that one lane does
         return true;
       };
-      auto taken = [&](uint64_t* bar) { tc_fence_before(); __syncwarp(); if (lane == 0) mbar_arrive_leader(bar); };
+      auto taken = [&](uint64_t* bar) { tc_fence_before(); __syncwarp(); if (lane == 0) mbar_arrive_leader(bar); __syncwarp(); };
       bool edge;
       if constexpr (ADD) {
         float x[PER][P::COLS];
@@ -315,16 +319,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FP8_THREADS, 1) fp8_
     while (gtime_ns() - t0 < 2000000ull) __nanosleep(1000);
     __syncthreads();
   }
+  __syncwarp();
   if (warp == 1) { tc_fence_after(); tmem_dealloc_pair(tmem, 512); }
 }
 
 // ------------------------------------------------------------------ host
 typedef void (*Fp8Fn)(Fp8Args);
-struct Fp8Variant { int tn, f32; Fp8Fn fn; int smem; };
-static const Fp8Variant g_fp8[] = {
-  {256, 0, fp8_pair_kernel<256, 5, bf16>, Fp8Smem<256, 5>::DYNAMIC}, {128, 0, fp8_pair_kernel<128, 7, bf16>, Fp8Smem<128, 7>::DYNAMIC}, {64, 0, fp8_pair_kernel<64, 8, bf16>, Fp8Smem<64, 8>::DYNAMIC},
-  {128, 1, fp8_pair_kernel<128, 7, float>, Fp8Smem<128, 7>::DYNAMIC}, {64, 1, fp8_pair_kernel<64, 8, float>, Fp8Smem<64, 8>::DYNAMIC},
-};
+struct Fp8Variant { int tn, ar, f32; Fp8Fn fn; int smem; };
+#define V_(TN, ST, AR, F, O) {TN, AR, F, fp8_pair_kernel<TN, ST, AR, O>, Fp8Smem<TN, ST, AR>::DYNAMIC}
+static const Fp8Variant g_fp8[] = {V_(256, 5, 128, 0, bf16), V_(128, 7, 128, 0, bf16), V_(64, 8, 128, 0, bf16), V_(64, 14, 64, 0, bf16),
+                                   V_(128, 7, 128, 1, float), V_(64, 8, 128, 1, float), V_(64, 14, 64, 1, float)};
+#undef V_
 static int g_fp8_pairs[64] = {0};
 
 static int fp8_ready(int dev) {
@@ -349,9 +354,8 @@ static int fp8_ready(int dev) {
 
 using namespace piccl_ops;
 
-constexpr int kFewRows = 64;
-static bool few_takes(const void* x, int fp32, long long stride, int M, long long K) {
-  return M <= kFewRows && !fp32 && K % 8 == 0 && stride % 8 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0;
+static bool few_takes(const void* x, int fp32, long long stride, int M, int N, long long K) {
+  return fp8_few_takes(M, N, K) && !fp32 && K % 8 == 0 && stride % 8 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0;
 }
 
 extern "C" {
@@ -361,14 +365,14 @@ int piccl_ops_fp8_gemm(const void* a, const void* sa, const void* b, const void*
   if (M <= 0 || N <= 0 || K <= 0 || K % 128 || K > 0x7fffff00ll || M > 0x7fffff00 || N > 0x7fffff00) return -1;
   for (const void* p : {a, sa, b, sb}) if (!p || (reinterpret_cast<uintptr_t>(p) & 15)) return -2;
   if (!out || (reinterpret_cast<uintptr_t>(out) & (f32 ? 3 : 1)) || (reinterpret_cast<uintptr_t>(bias) & 1)) return -2;
-  if (M <= kFewRows && !force_tn) return fp8_few(nullptr, 0, a, sa, b, sb, bias, out, f32, M, N, (int)K, 0, stream);
+  if (!force_tn && fp8_few_takes(M, N, K)) return fp8_few(nullptr, 0, a, sa, b, sb, bias, out, f32, M, N, (int)K, stream);
   int dev = 0; cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64) return -6;
   const int rc = fp8_ready(dev); if (rc) return rc;
   const long row_tiles = (M + 255) / 256;
   const Fp8Variant* v = nullptr; double best = 0;
   for (const Fp8Variant& c : g_fp8) {
-    if (c.f32 != (f32 != 0) || (force_tn && c.tn != force_tn)) continue;
+    if (c.f32 != (f32 != 0) || (force_tn && c.tn != force_tn) || (c.ar == 64) != (M <= 64 && c.tn <= 64)) continue;
     const long tiles = row_tiles * ((N + c.tn - 1) / c.tn);
     const double cost = (double)((tiles + g_fp8_pairs[dev] - 1) / g_fp8_pairs[dev]) * (c.tn == 256 ? 136 : c.tn == 128 ? 84 : 70);
     if (!v || cost < best) { v = &c; best = cost; }
@@ -379,7 +383,7 @@ int piccl_ops_fp8_gemm(const void* a, const void* sa, const void* b, const void*
   g.M = M; g.N = N; g.kb = (int)(K / 128); g.k4 = (g.kb + 3) / 4; g.bias = (const bf16*)bias; g.out = out;
   const int esz = f32 ? 4 : 2;
   g.store_tma = (size_t)N * esz % 16 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0;
-  if (!fp8_map(&g.ta, 1, a, M, K, FP8_BM, FP8_BK, true) || !fp8_map(&g.tb, 1, b, N, K, v->tn / 2, FP8_BK, true) ||
+  if (!fp8_map(&g.ta, 1, a, M, K, v->ar, FP8_BK, true) || !fp8_map(&g.tb, 1, b, N, K, v->tn / 2, FP8_BK, true) ||
       !fp8_map(&g.sa, 4, sa, (uint64_t)((M + 127) / 128) * g.k4, 128, 1, 128, false) || !fp8_map(&g.sb, 4, sb, (uint64_t)((N + 127) / 128) * g.k4, 128, 1, 128, false)) return -3;
   if (g.store_tma && !fp8_map(&g.tc, esz, out, M, N, 32, 128 / esz, true)) return -3;
   g.bias_words = reinterpret_cast<uintptr_t>(bias) % 16 == 0;
@@ -393,14 +397,14 @@ int piccl_ops_fp8_gemm(const void* a, const void* sa, const void* b, const void*
 
 // out [M, N] = x [M, K] w [N, K]^T + bias, x bf16 (or fp32) with rows `stride` elements apart; keep, keep_s: null, or room for x along its columns in 8 bits ([K, M up to 128]).
 // scratch, scratch_s: room for x in 8 bits, or null where piccl_ops_fp8_linear_scratch says 0.  Returns the number of launches, or a negative code.
-int piccl_ops_fp8_linear_scratch(const void* x, int fp32, long long stride, int M, long long K, int keep) { return keep || !few_takes(x, fp32, stride, M, K); }
+int piccl_ops_fp8_linear_scratch(const void* x, int fp32, long long stride, int M, int N, long long K, int keep) { return keep || !few_takes(x, fp32, stride, M, N, K); }
 int piccl_ops_fp8_linear(const void* x, int fp32, long long stride, const void* w, const void* sw, const void* bias, void* out, int f32, void* scratch, void* scratch_s, void* keep, void* keep_s, int M,
                          int N, long long K, void* stream) {
   if (M <= 0 || N <= 0 || K <= 0 || K > 0x7fffff00ll || stride < K) return -1;
-  if (!piccl_ops_fp8_linear_scratch(x, fp32, stride, M, K, keep != nullptr)) {
+  if (!piccl_ops_fp8_linear_scratch(x, fp32, stride, M, N, K, keep != nullptr)) {
     for (const void* p : {x, w, sw}) if (!p || (reinterpret_cast<uintptr_t>(p) & 15)) return -2;
     if (!out || (reinterpret_cast<uintptr_t>(out) & (f32 ? 3 : 1)) || (reinterpret_cast<uintptr_t>(bias) & 1)) return -2;
-    const int rc = fp8_few((const bf16*)x, stride, nullptr, nullptr, w, sw, bias, out, f32, M, N, (int)K, 0, stream);
+    const int rc = fp8_few((const bf16*)x, stride, nullptr, nullptr, w, sw, bias, out, f32, M, N, (int)K, stream);
     return rc ? rc : 1;
   }
   if (!scratch || !scratch_s) return -2;

@@ -28,7 +28,7 @@ int piccl_ops_attn_parts(int B, int S);
 int piccl_ops_attn_bwd(const void* qkv, const void* out, const void* dout, const float* lse, float* scratch, void* dqkv, float* part, int B, int S, int H, void* stream);
 int piccl_ops_fp8_quantize(const void* x, int fp32, long long R, long long C, long long stride, void* q, void* qs, void* t, void* ts, int square, void* stream);
 int piccl_ops_fp8_gemm(const void* a, const void* sa, const void* b, const void* sb, const void* bias, void* out, int f32, int M, int N, long long K, int force_tn, void* stream);
-int piccl_ops_fp8_linear_scratch(const void* x, int fp32, long long stride, int M, long long K, int keep);
+int piccl_ops_fp8_linear_scratch(const void* x, int fp32, long long stride, int M, int N, long long K, int keep);
 int piccl_ops_fp8_linear(const void* x, int fp32, long long stride, const void* w, const void* sw, const void* bias, void* out, int f32, void* scratch, void* scratch_s, void* keep, void* keep_s, int M, int N, long long K, void* stream);
 #ifdef __cplusplus
 }

@@ -101,7 +101,7 @@ PyObject* linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const int M = (int)x->size(0), fp32 = x->scalar_type() == at::kFloat, f32 = out->scalar_type() == at::kFloat;
     const long long K = x->size(1), stride = row_stride(*x);
     int rc;
-    if (piccl_ops_fp8_linear_scratch(x->data_ptr(), fp32, stride, M, K, keep.v != nullptr)) {
+    if (piccl_ops_fp8_linear_scratch(x->data_ptr(), fp32, stride, M, (int)out->size(1), K, keep.v != nullptr)) {
       const Scratch q(M, K);
       rc = piccl_ops_fp8_linear(x->data_ptr(), fp32, stride, ptr(w.v), ptr(w.s), ptr(bias), out->data_ptr(), f32, q.v, q.s, ptr(keep.v), ptr(keep.s), M, (int)out->size(1), K, stream());
     } else

@@ -63,7 +63,7 @@ def test_quantize(rows, cols, dtype, square, copies):
         _same(t, x.t(), square)
 
 
-@pytest.mark.parametrize("M,N,K", [(1, 1, 1), (1, 256, 128), (128, 128, 128), (256, 256, 512), (255, 257, 384), (300, 520, 1000), (129, 64, 4096), (2331, 768, 200), (64, 50257, 768), (1000, 72, 640)])
+@pytest.mark.parametrize("M,N,K", [(1, 1, 1), (1, 256, 128), (128, 128, 128), (256, 256, 512), (255, 257, 384), (300, 520, 1000), (129, 64, 4096), (2331, 768, 200), (64, 50257, 768), (1000, 72, 640), (48, 1000, 2048), (33, 97, 1152)])
 @pytest.mark.parametrize("tile", [0, 64, 128, 256])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_product(M, N, K, tile, dtype):
