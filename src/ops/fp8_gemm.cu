@@ -355,7 +355,7 @@ static int fp8_ready(int dev) {
 using namespace piccl_ops;
 
 static bool few_takes(const void* x, int fp32, long long stride, int M, int N, long long K) {
-  return fp8_few_takes(M, N, K) && !fp32 && K % 8 == 0 && stride % 8 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0;
+  return fp8_few_takes(M, N, K, false) && !fp32 && K % 8 == 0 && stride % 8 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0;
 }
 
 extern "C" {
@@ -365,7 +365,7 @@ int piccl_ops_fp8_gemm(const void* a, const void* sa, const void* b, const void*
   if (M <= 0 || N <= 0 || K <= 0 || K % 128 || K > 0x7fffff00ll || M > 0x7fffff00 || N > 0x7fffff00) return -1;
   for (const void* p : {a, sa, b, sb}) if (!p || (reinterpret_cast<uintptr_t>(p) & 15)) return -2;
   if (!out || (reinterpret_cast<uintptr_t>(out) & (f32 ? 3 : 1)) || (reinterpret_cast<uintptr_t>(bias) & 1)) return -2;
-  if (!force_tn && fp8_few_takes(M, N, K)) return fp8_few(nullptr, 0, a, sa, b, sb, bias, out, f32, M, N, (int)K, stream);
+  if (!force_tn && fp8_few_takes(M, N, K, true)) return fp8_few(nullptr, 0, a, sa, b, sb, bias, out, f32, M, N, (int)K, stream);
   int dev = 0; cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64) return -6;
   const int rc = fp8_ready(dev); if (rc) return rc;

@@ -89,8 +89,8 @@ def test_product(M, N, K, tile, dtype):
     assert torch.isnan(guard[M]).all()
 
 
-@pytest.mark.parametrize("M", [1, 2, 15, 16, 17, 31, 33, 64, 65])
-@pytest.mark.parametrize("N,K", [(1, 8), (128, 128), (257, 640), (1000, 1096), (4096, 1024), (520, 4104), (136, 72), (64, 333)])
+@pytest.mark.parametrize("M", [1, 2, 7, 8, 9, 15, 16, 17, 23, 25, 31, 32, 33, 64, 65])
+@pytest.mark.parametrize("N,K", [(1, 8), (128, 128), (257, 640), (1000, 1096), (4096, 1024), (520, 4104), (136, 72), (64, 333), (5000, 264), (64, 8192)])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_linear_of_few_rows(M, N, K, dtype):
     """One launch up to 64 rows where they lie on 16-byte boundaries: the same bits as the quantiser and a product in 64 bits, within that product's bound."""
