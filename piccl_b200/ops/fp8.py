@@ -51,6 +51,9 @@ class Fp8(NamedTuple):
 
 def empty(rows: int, cols: int, device="cuda") -> Fp8:
     """Room for a matrix of `rows` by `cols`."""
+    fast = _native_calls()
+    if fast and (t := fast.empty(rows, cols, device)):
+        return Fp8(*t)
     blocks = (cols + 127) // 128
     return Fp8(torch.empty(rows, blocks * 128, dtype=E4M3, device=device), torch.empty((rows + 127) // 128, (blocks + 3) // 4, 32, 4, 4, dtype=torch.uint8, device=device))
 

@@ -21,7 +21,7 @@ from typing import Optional, Sequence, Union
 import torch
 
 from . import _bump, _s
-from .fp8 import E4M3, _on
+from .fp8 import E4M3, _native_calls, _on
 from .gemm_sm100 import _native, _ptr
 
 _DECAY, _P_F32, _G_F32, _WORDS = 1, 2, 4, 8
@@ -64,6 +64,10 @@ class AdamW:
         self.step_dev, self._ticket = zeros(1, torch.int32), zeros(1, torch.int32)
         self._table = None
         self.set_grads(grads)
+        fast = _native_calls()
+        self._fast = fast.adamw_step if fast else None
+        self._handle = fast.adamw(self.device.index, self._table.data_ptr(), self._count, block, bits == 8, self.m.data_ptr(), self.v.data_ptr(), _ptr(self.m_scales) or 0, _ptr(self.v_scales) or 0,
+                                  self.step_dev.data_ptr(), self._ticket.data_ptr(), self.seed) if fast else None
 
     def set_grads(self, grads: Sequence[torch.Tensor]) -> None:
         """Other tensors to take the gradients from, from the next step on (a copy of addresses to the device; not within a capture)."""
@@ -91,6 +95,9 @@ class AdamW:
 
     def step(self, lr: float, b1: float = 0.9, b2: float = 0.95, eps: float = 1e-8, wd: float = 0.1, gscale: Union[float, torch.Tensor] = 1.0) -> None:
         """One step from the gradients as they are now."""
+        if self._fast is not None and self._fast(self._handle, lr, b1, b2, eps, wd, gscale):
+            _bump()
+            return
         if not (0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0):
             raise ValueError(f"AdamW: decay rates of the moments are in [0, 1), not {b1} and {b2}")
         dev = None

@@ -22,7 +22,7 @@ enum { ADAM_DECAY = 1, ADAM_P_F32 = 2, ADAM_G_F32 = 4, ADAM_WORDS = 8 };      //
 struct AdamArgs {
   const AdamTensor* tensors; int count; long long blocks;
   void *m, *v; uint8_t *ms, *vs;
-  float lr, b1, c1, b2, c2, eps, wd; double lb1, lb2;      // c: 1 - b; lb: logarithms
+  float lr, b1, c1, b2, c2, eps, wd, lb1, lb2;      // c: 1 - b; lb: logarithms
   float gscale; const float* gscale_dev;
   int* step; unsigned* ticket; uint32_t seed;
 };
@@ -146,8 +146,8 @@ struct AdamStep {
     __shared__ float s_c[2];
     const int t = *(volatile int*)a.step + 1;
     if (threadIdx.x == 0) {
-      s_c[0] = (float)(1.0 / -expm1(t * a.lb1));
-      s_c[1] = (float)(1.0 / sqrt(-expm1(t * a.lb2)));
+      s_c[0] = 1.f / -expm1f((float)t * a.lb1);             // 1 - b^t without cancellation
+      s_c[1] = 1.f / sqrtf(-expm1f((float)t * a.lb2));
     }
     __syncthreads();
     rc2 = s_c[1]; lr1 = a.lr * s_c[0];
@@ -261,6 +261,12 @@ __global__ void __launch_bounds__(256, 3) adamw_many8_kernel(const AdamArgs a) {
       load_words(now.master + i, w);
       if (now.flags & ADAM_G_F32) load_words(gradients(now, i), gw); else load_words(gradients(now, i), reinterpret_cast<uint32_t (&)[E / 2]>(gw));
     } else load_some(gradients(now, i), now.master + i, left, now.flags, gw, w);
+    if (block + stride < now.end && l < 8) {                // the next block on its way into L2, a line of 128 bytes a lane
+      const long long next = block + stride, j = (next - now.first) * 128;
+      const char* const at = l < 4 ? reinterpret_cast<const char*>(now.master + j) + l * 128 : l < 6 ? static_cast<const char*>(gradients(now, j)) + (l - 4) * 128
+                             : (l == 6 ? static_cast<const char*>(a.m) : static_cast<const char*>(a.v)) + next * 128;
+      asm volatile("prefetch.global.L2 [%0];" ::"l"(at));
+    }
     f32x2 m[4], v[4], root[4];
 #pragma unroll
     for (int k = 0; k < 2; k++) {
@@ -305,7 +311,7 @@ int piccl_ops_adamw_many(const void* tensors, int count, long long blocks, int b
   if (count < 0 || blocks < 0 || !(b1 >= 0 && b1 < 1) || !(b2 >= 0 && b2 < 1)) return -1;
   if ((blocks && (!tensors || !m || !v || (bits8 && (!ms || !vs)))) || !step || !ticket) return -2;
   if ((reinterpret_cast<uintptr_t>(m) | reinterpret_cast<uintptr_t>(v)) & 15) return -2;
-  AdamArgs a{static_cast<const AdamTensor*>(tensors), count, blocks, m, v, (uint8_t*)ms, (uint8_t*)vs, lr, (float)b1, (float)(1 - b1), (float)b2, (float)(1 - b2), eps, wd, log(b1), log(b2),
+  AdamArgs a{static_cast<const AdamTensor*>(tensors), count, blocks, m, v, (uint8_t*)ms, (uint8_t*)vs, lr, (float)b1, (float)(1 - b1), (float)b2, (float)(1 - b2), eps, wd, (float)log(b1), (float)log(b2),
              gscale, gscale_dev, step, ticket, seed};
   const long long want = bits8 ? (blocks + 15) / 16 : (blocks + 7) / 8, most = 148 * (bits8 ? 3 : 5);
   const dim3 grid((unsigned)(want < 1 ? 1 : want < most ? want : most));

@@ -1,13 +1,15 @@
-// The 8-bit layers (piccl_b200/ops/fp8.py) as native functions that take tensors.
+// The 8-bit layers (piccl_b200/ops/fp8.py) and the step of the optimiser over many tensors (optimizer.py) as native functions that take tensors.
 //
 // A layer is one or two launches of a few microseconds; checked and issued from Python through ctypes it took 23 us of host time, most of it the checks, the allocation of
 // scratch and the conversion of arguments.  Each function here returns the number of launches, or 0 if anything about its arguments is not as it has to be (or nothing is to be launched): the
 // Python function then looks at them itself and says what is wrong.
 #include <Python.h>
+#include <new>
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <torch/csrc/Device.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include "../ops/piccl_ops.h"
 
@@ -135,8 +137,54 @@ PyObject* linear_bwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
+// empty(rows, cols, device): values and scales; None if they cannot be made here
+PyObject* empty(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    if (n != 3 || !THPDevice_Check(a[2])) Py_RETURN_NONE;
+    const int64_t rows = PyLong_AsLongLong(a[0]), cols = PyLong_AsLongLong(a[1]);
+    if (PyErr_Occurred()) return nullptr;
+    if (rows < 0 || cols < 0) Py_RETURN_NONE;
+    const auto opt = at::TensorOptions().device(reinterpret_cast<THPDevice*>(a[2])->device);
+    const int64_t blocks = (cols + 127) / 128;
+    PyObject* const v = THPVariable_Wrap(at::empty({rows, blocks * 128}, opt.dtype(at::kFloat8_e4m3fn)));
+    PyObject* const s = v ? THPVariable_Wrap(at::empty({(rows + 127) / 128, (blocks + 3) / 4, 32, 4, 4}, opt.dtype(at::kByte))) : nullptr;
+    PyObject* const t = s ? PyTuple_Pack(2, v, s) : nullptr;
+    Py_XDECREF(v); Py_XDECREF(s);
+    return t;
+  });
+}
+
+// What stays the same from step to step of an optimiser
+struct Adam { int device, count, bits8; long long blocks; void *table, *m, *v, *ms, *vs, *step, *ticket; unsigned seed; };
+// adamw(device, table, count, blocks, bits8, m, v, ms, vs, step, ticket, seed), all numbers -> handle
+PyObject* adamw(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  long long x[12];
+  if (n != 12) { PyErr_SetString(PyExc_TypeError, "adamw: 12 numbers"); return nullptr; }
+  for (int i = 0; i < 12; i++) { x[i] = (long long)PyLong_AsUnsignedLongLongMask(a[i]); if (PyErr_Occurred()) return nullptr; }
+  auto p = [&](int i) { return reinterpret_cast<void*>(x[i]); };
+  Adam* const h = new (std::nothrow) Adam{(int)x[0], (int)x[2], (int)x[4], x[3], p(1), p(5), p(6), p(7), p(8), p(9), p(10), (unsigned)x[11]};
+  return h ? PyCapsule_New(h, "adamw", [](PyObject* c) { delete static_cast<Adam*>(PyCapsule_GetPointer(c, "adamw")); }) : PyErr_NoMemory();
+}
+// adamw_step(handle, lr, b1, b2, eps, wd, gscale): gscale a number or a tensor; 0 if that tensor is not one fp32 value on the device
+PyObject* adamw_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    if (n != 7) return no();
+    const Adam* const h = static_cast<const Adam*>(PyCapsule_GetPointer(a[0], "adamw"));
+    if (!h) return nullptr;
+    double x[5], g = 1.0;
+    for (int i = 0; i < 5; i++) { x[i] = PyFloat_AsDouble(a[1 + i]); if (PyErr_Occurred()) return nullptr; }
+    const at::Tensor* const t = tensor(a[6]);
+    if (!t) { g = PyFloat_AsDouble(a[6]); if (PyErr_Occurred()) return nullptr; }
+    else if (t->scalar_type() != at::kFloat || t->numel() != 1 || !t->is_cuda() || t->device().index() != h->device) return no();
+    if (!(x[1] >= 0 && x[1] < 1 && x[2] >= 0 && x[2] < 1)) return no();
+    const c10::cuda::CUDAGuard guard((c10::DeviceIndex)h->device);
+    return answer(piccl_ops_adamw_many(h->table, h->count, h->blocks, h->bits8, h->m, h->v, h->ms, h->vs, (float)x[0], x[1], x[2], (float)x[3], (float)x[4], (float)g,
+                                       t ? t->data_ptr<float>() : nullptr, static_cast<int*>(h->step), static_cast<unsigned*>(h->ticket), h->seed, stream()), 1, "adamw_many");
+  });
+}
+
 #define M_(f) {#f, (PyCFunction)(void (*)(void))f, METH_FASTCALL, nullptr}
-PyMethodDef methods[] = {M_(quantize), M_(product), M_(linear), M_(linear_bwd), {nullptr, nullptr, 0, nullptr}};
+PyMethodDef methods[] = {M_(quantize), M_(product), M_(linear), M_(linear_bwd), M_(empty), M_(adamw), M_(adamw_step), {nullptr, nullptr, 0, nullptr}};
 #undef M_
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_tensorcall", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
