@@ -33,6 +33,7 @@ import torch
 from .. import _native as N
 from .. import ops
 from ..ops import gemm
+from ..ops.optimizer import AdamW
 
 _READY = C.CFUNCTYPE(None, C.c_longlong)
 _MAX_GRAPHS = 8
@@ -79,7 +80,10 @@ _NODECAY = ("ln1_g", "ln1_b", "b_qkv", "b_o", "ln2_g", "ln2_b", "b_fc", "b_proj"
 
 
 class GPT2:
-    def __init__(self, cfg: GPT2Config, device="cuda", seed: int = 0):
+    def __init__(self, cfg: GPT2Config, device="cuda", seed: int = 0, adam_bits: int = 32):
+        """adam_bits: 32, or 8 for moments of the optimiser at a byte an element (ops/optimizer.py)."""
+        if adam_bits not in (8, 32):
+            raise ValueError(f"moments of 8 or 32 bits, not {adam_bits}")
         self.cfg = cfg
         self.device = torch.device(device)
         D, L, Vp, S = cfg.d_model, cfg.n_layer, cfg.padded_vocab, cfg.seq_len
@@ -112,10 +116,16 @@ class GPT2:
         self.n_params = total
         self._init_weights(seed)
         self.master = self.flat_p.float()
-        self.m = torch.zeros_like(self.master)
-        self.v = torch.zeros_like(self.master)
         self.step_count = 0
-        self.step_dev = torch.zeros(1, dtype=torch.int32, device=self.device)     # the same counter on the device (graph replay)
+        self._adam = None
+        if adam_bits == 8:
+            pieces = [slice(b, e) for b, e, _ in self.groups]
+            self._adam = AdamW([self.flat_p[c] for c in pieces], [self.flat_g[c] for c in pieces], [self.master[c] for c in pieces], bits=8, decay=[d for _, _, d in self.groups], seed=seed)
+            self.m, self.v, self.step_dev = self._adam.m, self._adam.v, self._adam.step_dev
+        else:
+            self.m = torch.zeros_like(self.master)
+            self.v = torch.zeros_like(self.master)
+            self.step_dev = torch.zeros(1, dtype=torch.int32, device=self.device)     # the same counter on the device (graph replay)
         # decaying and non-decaying runs alternate; their ends in packs of 8 elements
         self._run_ends = torch.tensor([e // 8 for _, e, _ in self.groups], dtype=torch.int32, device=self.device)
         self._ticket = torch.zeros(1, dtype=torch.int32, device=self.device)
@@ -266,6 +276,9 @@ class GPT2:
         """Fused AdamW over the flat buffers in one launch (one per run of parameters in models of more than some 500 layers); the step number lives
         on the device so that it can be replayed."""
         self.step_count += 1
+        if self._adam is not None:
+            self._adam.step(lr, betas[0], betas[1], eps, weight_decay)
+            return
         if len(self.groups) > ops.MAX_ADAMW_RUNS:
             self.step_dev.add_(1)
             for b, e, decay in self.groups:

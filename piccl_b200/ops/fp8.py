@@ -1,7 +1,7 @@
 """Linear layers in 8 bits: the quantiser and the products of src/ops/fp8_quant.cu and fp8_gemm.cu.
 
 A matrix in 8 bits (`Fp8`) is e4m3 values, rows filled with zeros to a multiple of 128, and one power of two for each block of 128
-values of a row: byte e stands for 2^(e - 127), the smallest for which the block's largest finite magnitude is at most 448.  Values that
+values of a row: byte e, 1 to 254, stands for 2^(e - 127), the smallest for which the block's largest finite magnitude is at most 448.  Values that
 are not finite become NaN.  A product sums along the rows of both operands, so a matrix that two products sum over different
 dimensions is kept twice, the second time transposed; `square` gives both copies of a weight the same values.
 

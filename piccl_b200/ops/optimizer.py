@@ -51,6 +51,9 @@ class AdamW:
             for t in (p,) if w is None else (p, w):
                 if not t.is_contiguous() or not t.is_cuda or t.device != self.device:
                     raise ValueError("AdamW: contiguous tensors of one CUDA device wanted")
+        written = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in (*params, *(w for w in masters if w is not None)) if t.numel())
+        if any(a[1] > b[0] for a, b in zip(written, written[1:])):
+            raise ValueError("AdamW: parameters or masters that overlap")
         self.params, self.masters, self.decay, self.bits, self.seed = params, masters, [bool(d) for d in decay], bits, int(seed) & 0xFFFFFFFF
         self.places, block = [], 0                    # (first element in m and v, elements) of each tensor
         for p in params:

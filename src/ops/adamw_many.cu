@@ -261,8 +261,8 @@ __global__ void __launch_bounds__(256, 3) adamw_many8_kernel(const AdamArgs a) {
       load_words(now.master + i, w);
       if (now.flags & ADAM_G_F32) load_words(gradients(now, i), gw); else load_words(gradients(now, i), reinterpret_cast<uint32_t (&)[E / 2]>(gw));
     } else load_some(gradients(now, i), now.master + i, left, now.flags, gw, w);
-    if (block + stride < now.end && l < 8) {                // the next block on its way into L2, a line of 128 bytes a lane
-      const long long next = block + stride, j = (next - now.first) * 128;
+    const long long next = block + stride, j = (next - now.first) * 128;
+    if (j + 128 <= now.n && l < 8) {                        // the next block, if it is a whole one of this tensor, on its way into L2: a line of 128 bytes a lane
       const char* const at = l < 4 ? reinterpret_cast<const char*>(now.master + j) + l * 128 : l < 6 ? static_cast<const char*>(gradients(now, j)) + (l - 4) * 128
                              : (l == 6 ? static_cast<const char*>(a.m) : static_cast<const char*>(a.v)) + next * 128;
       asm volatile("prefetch.global.L2 [%0];" ::"l"(at));

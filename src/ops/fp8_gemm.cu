@@ -377,7 +377,7 @@ int piccl_ops_fp8_gemm(const void* a, const void* sa, const void* b, const void*
     const double cost = (double)((tiles + g_fp8_pairs[dev] - 1) / g_fp8_pairs[dev]) * (c.tn == 256 ? 136 : c.tn == 128 ? 84 : 70);
     if (!v || cost < best) { v = &c; best = cost; }
   }
-  if (!v) return -1;
+  if (!v || (double)row_tiles * ((N + v->tn - 1) / v->tn) > 0x7fffffff) return -1;
   Fp8Args g;
   memset(&g, 0, sizeof g);
   g.M = M; g.N = N; g.kb = (int)(K / 128); g.k4 = (g.kb + 3) / 4; g.bias = (const bf16*)bias; g.out = out;

@@ -31,12 +31,14 @@ def _tensors(sizes, master, grad, offset=0, seed=0, scale=1e-3):
 
 
 def _reference(w, m, v, g, t, decay, gscale=1.0, lr=0.0, b1=0.0, b2=0.0, eps=0.0, wd=0.0):
-    """The formula in fp64"""
+    """The formula in fp64, and the size of what is taken off a weight as its roundings count it: the sum that gives m may cancel, its addends' roundings do not.  These are some 16 half steps of fp32:
+    three of m, as many of each of 1 - b^t and its reciprocal, one of lr, two of an approximate root, one of eps, four of a quotient that is right to two steps."""
     g = g.double() * gscale
+    size = lr * (b1 * m.double().abs() + (1 - b1) * g.abs()) / (1 - b1 ** t)
     m = b1 * m.double() + (1 - b1) * g
     v = b2 * v.double() + (1 - b2) * g * g
-    w = w.double() * (1 - lr * (wd if decay else 0.0)) - lr * (m / (1 - b1 ** t)) / ((v / (1 - b2 ** t)).sqrt() + eps)
-    return w, m, v
+    below = (v / (1 - b2 ** t)).sqrt() + eps
+    return w.double() * (1 - lr * (wd if decay else 0.0)) - lr * (m / (1 - b1 ** t)) / below, m, v, size / below
 
 
 def _near(got, want, old, steps, change):
@@ -61,11 +63,10 @@ def test_moments_in_32_bits(master, grad, offset):
         for i, (w, m, v) in enumerate(before):
             want = _reference(w, m, v, grads[i], step, decay[i], 0.7, **RATES)
             got = opt.moments(i)
-            # m and v: two products and a sum, the gradient's scaling before; w: ten operations in the update, whose size is at most some lr
+            # m and v: two products and a sum, the gradient's scaling before
             _near(got[0], want[1], m, 4, grads[i].double().abs())
             _near(got[1], want[2], v, 6, (grads[i].double()) ** 2)
-            update = (want[0] - w.double()).abs()
-            _near(weights[i], want[0], w, 2, 10 * update)
+            _near(weights[i], want[0], w, 2, 10 * want[3])
             if master:
                 assert torch.equal(params[i], weights[i].to(torch.bfloat16))
 
@@ -132,7 +133,7 @@ def test_moments_in_8_bits(master, grad, offset):
                 same |= got == q.view(-1)
                 assert bool(same.all())
             want = _reference(w, m, v, grads[i], step, True, 0.7, **RATES)
-            _near(weights[i], want[0], w, 2, 10 * (want[0] - w.double()).abs())
+            _near(weights[i], want[0], w, 2, 10 * want[3])
             if master:
                 assert torch.equal(params[i], weights[i].to(torch.bfloat16))
 
@@ -210,5 +211,58 @@ def test_more_tensors_than_blocks_and_other_gradients():
     opt.set_grads(others)
     opt.step(**RATES)
     w0, g0 = torch.cat(before), torch.cat(others)
-    want = _reference(w0, torch.zeros_like(w0), torch.zeros_like(w0), g0, 1, True, **RATES)[0]
-    _near(torch.cat(params), want, w0, 2, 10 * (want - w0.double()).abs())
+    want = _reference(w0, torch.zeros_like(w0), torch.zeros_like(w0), g0, 1, True, **RATES)
+    _near(torch.cat(params), want[0], w0, 2, 10 * want[3])
+
+
+def test_gpt2_with_moments_in_8_bits():
+    """The first step is that of moments in 32 bits (nothing has been rounded before it), and replayed steps of the trainer are those issued one by one."""
+    from piccl_b200.models.gpt2 import GPT2, GPT2Config
+    from piccl_b200.train import DataParallelTrainer
+    cfg = GPT2Config.tiny()
+    tok = torch.randint(0, cfg.vocab_size, (2, cfg.seq_len + 1), generator=torch.Generator().manual_seed(0))
+    a, b = tok[:, :-1].contiguous(), tok[:, 1:].contiguous()
+    models = [GPT2(cfg, seed=3, adam_bits=bits) for bits in (32, 8)]
+    for m in models:
+        m.forward_backward(a.cuda(), b.cuda())
+    assert torch.equal(models[0].flat_g, models[1].flat_g)
+    before = models[0].master.clone()
+    for m in models:
+        m.optimizer_step(lr=1e-3)
+    w32, w8 = (m.master.double() for m in models)
+    _near(models[1].master, w32, before, 4, 20 * (w32 - before.double()).abs())
+    assert torch.equal(models[1].flat_p, models[1].master.to(torch.bfloat16)) and int(models[1].step_dev) == 1
+    runs = []
+    for graph in (False, True):
+        tr = DataParallelTrainer(cfg, None, seed=3, adam_bits=8, use_graph=graph)
+        losses = [tr.step(a.pin_memory(), b.pin_memory()) for _ in range(5)]
+        assert int(tr.model.step_dev) == tr.model.step_count == 5
+        runs.append((losses, tr.model.master.clone(), tr.model.m.float()))
+    assert all(math.isfinite(x) for x in runs[0][0] + runs[1][0])
+    with pytest.raises(ValueError):
+        GPT2(cfg, adam_bits=16)
+
+
+def test_refusals_on_the_gpu():
+    from piccl_b200.ops.optimizer import AdamW
+    p, g = torch.ones(16, device="cuda"), torch.ones(16, device="cuda")
+    opt = AdamW([p], [g])
+    for kw in (dict(b1=1.0), dict(b2=-0.5), dict(gscale=torch.ones(2, device="cuda")), dict(gscale=torch.ones(1)), dict(gscale=torch.ones(1, device="cuda", dtype=torch.float64))):
+        with pytest.raises(ValueError):
+            opt.step(1e-3, **kw)
+    for grads in ([], [g[:8]], [g.double()], [g.cpu()], [torch.ones(32, device="cuda")[::2]]):
+        with pytest.raises(ValueError):
+            opt.set_grads(grads)
+    for params in ([p, p], [p, p[8:]], [p[:9], p[8:]]):
+        with pytest.raises(ValueError, match="overlap"):
+            AdamW(params, [torch.zeros_like(t) for t in params])
+    assert int(opt.step_dev) == 0 and bool((p == 1).all())
+    graph = torch.cuda.CUDAGraph()
+    opt.step(0.0, wd=0.0)
+    with torch.cuda.graph(graph):
+        with pytest.raises(RuntimeError):
+            opt.set_grads([g])
+        opt.step(0.0, wd=0.0)
+    none = AdamW([torch.empty(0, device="cuda")], [torch.empty(0, device="cuda")], bits=8)
+    none.step(1e-3)
+    assert int(none.step_dev) == 1
