@@ -213,8 +213,7 @@ __global__ void __launch_bounds__(256, 5) adamw_many_kernel(const AdamArgs a) {
   const AdamStep step(a);
   const int l = threadIdx.x & 31;
   const long long stride = gridDim.x * 8ll;
-  AdamNow now;
-  now.at = 0; now.end = -1;
+  AdamNow now = {nullptr, nullptr, nullptr, 0, 0, -1, 0, 0};
   for (long long block = blockIdx.x * 8ll + (threadIdx.x >> 5); block < a.blocks; block += stride) {
     if (block >= now.end) adam_find(a, block, now);
     const long long i = (block - now.first) * 128 + l * E, s = block * 128 + l * E;
@@ -243,8 +242,7 @@ __global__ void __launch_bounds__(256, 3) adamw_many8_kernel(const AdamArgs a) {
   const AdamStep step(a);
   const int l = threadIdx.x & 15, second = threadIdx.x >> 4 & 1;
   const long long stride = gridDim.x * 16ll;
-  AdamNow now;
-  now.at = 0; now.end = -1;
+  AdamNow now = {nullptr, nullptr, nullptr, 0, 0, -1, 0, 0};
   for (long long block = blockIdx.x * 16ll + (threadIdx.x >> 4); block - second < a.blocks; block += stride) {
     const bool there = block < a.blocks;                    // the first half of a warp may have the last block
     if (there && block >= now.end) adam_find(a, block, now);

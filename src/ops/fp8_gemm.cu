@@ -61,7 +61,8 @@ template <> struct OutPiece<float> {
 };
 // Rows of a result that do not start on 16 bytes, which no TMA store takes: a warp writes a row at a time, a word of 4 bytes a lane, from words of 16 rows that it has loaded (row by row, each
 // waiting for its load, a row took 200 clocks).  Rows of bf16 that begin in the middle of a word are moved by half a word, their first and last value written on their own.
-// left: columns that are there.
+// 2331 x 50257 x 768: 150 us, where 50256 columns take 105.  What that costs are the sectors of which a piece writes a part: rows moved to 16-byte pieces in shared memory took 157, the ends of the pieces
+// alone 155, all but the ends 141.  left: columns that are there.
 __device__ __forceinline__ uint32_t staged_word(const uint8_t* staging, int r, int lane) {
   return *reinterpret_cast<const uint32_t*>(staging + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4);
 }

@@ -89,6 +89,27 @@ def test_product(M, N, K, tile, dtype):
     assert torch.isnan(guard[M]).all()
 
 
+@pytest.mark.parametrize("offset", [0, 1, 2, 3, 4, 5, 6, 7])
+@pytest.mark.parametrize("N", [61, 64, 67, 126, 137, 264, 521])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_results_at_any_address(offset, N, dtype):
+    """Rows that begin anywhere in a 16-byte word, as a result's does that lies within a buffer: the same bits as in a buffer of its own, and nothing beside it."""
+    from piccl_b200.ops import fp8
+    M, K = 203, 256
+    a, b = fp8.empty(M, K), fp8.empty(N, K)
+    fp8.quantize(_randn(M, K, seed=1), a)
+    fp8.quantize(_randn(N, K, seed=2), b)
+    wide = fp8.empty((N + 7) // 8 * 8, K)
+    fp8.quantize(torch.cat([_randn(N, K, seed=2), torch.zeros(-N % 8, K, dtype=torch.bfloat16, device="cuda")]), wide)
+    want = torch.empty(M, (N + 7) // 8 * 8, dtype=dtype, device="cuda")
+    fp8.product(a, wide, want)
+    for tile in (64, 128, 256):
+        buf = torch.full((M * N + 16,), math.nan, dtype=dtype, device="cuda")
+        fp8.product(a, b, buf[offset:offset + M * N].view(M, N), _tile=min(tile, 128) if dtype == torch.float32 else tile)
+        assert torch.equal(buf[offset:offset + M * N].view(M, N), want[:, :N])
+        assert bool(buf[:offset].isnan().all()) and bool(buf[offset + M * N:].isnan().all())
+
+
 @pytest.mark.parametrize("M", [1, 2, 7, 8, 9, 15, 16, 17, 23, 25, 31, 32, 33, 64, 65])
 @pytest.mark.parametrize("N,K", [(1, 8), (128, 128), (257, 640), (1000, 1096), (4096, 1024), (520, 4104), (136, 72), (64, 333), (5000, 264), (64, 8192)])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
