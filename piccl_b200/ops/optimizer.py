@@ -25,7 +25,7 @@ from .fp8 import E4M3, _native_calls, _on
 from .gemm_sm100 import _native, _ptr
 
 _DECAY, _P_F32, _G_F32, _WORDS = 1, 2, 4, 8
-_STEP = [C.c_void_p, C.c_int, C.c_longlong, C.c_int] + [C.c_void_p] * 4 + [C.c_float, C.c_double, C.c_double] + [C.c_float] * 3 + [C.c_void_p] * 3 + [C.c_uint, C.c_void_p]
+_STEP = [C.c_void_p, C.c_void_p, C.c_longlong, C.c_int] + [C.c_void_p] * 4 + [C.c_float, C.c_double, C.c_double] + [C.c_float] * 3 + [C.c_void_p] * 3 + [C.c_uint, C.c_void_p]
 
 
 class _Tensor(C.Structure):          # AdamTensor of src/ops/adamw_many.cu
@@ -65,11 +65,13 @@ class AdamW:
         self.m, self.v = zeros(block * 128, kind), zeros(block * 128, kind)
         self.m_scales, self.v_scales = (torch.ones(block, dtype=torch.uint8, device=self.device) for _ in range(2)) if bits == 8 else (None, None)
         self.step_dev, self._ticket = zeros(1, torch.int32), zeros(1, torch.int32)
+        lengths = [(n + 127) // 128 for _, n in self.places if n]
+        self._owner = torch.repeat_interleave(torch.arange(len(lengths), dtype=torch.int32), torch.tensor(lengths, dtype=torch.int64)).to(self.device)      # the tensor of each block
         self._table = None
         self.set_grads(grads)
         fast = _native_calls()
         self._fast = fast.adamw_step if fast else None
-        self._handle = fast.adamw(self.device.index, self._table.data_ptr(), self._count, block, bits == 8, self.m.data_ptr(), self.v.data_ptr(), _ptr(self.m_scales) or 0, _ptr(self.v_scales) or 0,
+        self._handle = fast.adamw(self.device.index, self._table.data_ptr(), self._owner.data_ptr(), block, bits == 8, self.m.data_ptr(), self.v.data_ptr(), _ptr(self.m_scales) or 0, _ptr(self.v_scales) or 0,
                                   self.step_dev.data_ptr(), self._ticket.data_ptr(), self.seed) if fast else None
 
     def set_grads(self, grads: Sequence[torch.Tensor]) -> None:
@@ -89,7 +91,7 @@ class AdamW:
             if all(t is None or t.data_ptr() % (8 * t.element_size()) == 0 for t in (p, w, g)):
                 flags |= _WORDS
             records.append(_Tensor(p.data_ptr(), 0 if w is None else w.data_ptr(), g.data_ptr(), n, first // 128, flags, 0))
-        self.grads, self._count = grads, len(records)
+        self.grads = grads
         raw = torch.frombuffer(bytearray((_Tensor * max(1, len(records)))(*records)), dtype=torch.uint8)
         if self._table is None:
             self._table = raw.to(self.device)
@@ -109,7 +111,7 @@ class AdamW:
                 raise ValueError("AdamW: gscale is a number or one fp32 value on the device of the parameters")
             gscale, dev = 1.0, gscale
         with _on(self.device):
-            rc = _native("piccl_ops_adamw_many", _STEP)(self._table.data_ptr(), self._count, self.blocks, self.bits == 8, self.m.data_ptr(), self.v.data_ptr(), _ptr(self.m_scales),
+            rc = _native("piccl_ops_adamw_many", _STEP)(self._table.data_ptr(), self._owner.data_ptr(), self.blocks, self.bits == 8, self.m.data_ptr(), self.v.data_ptr(), _ptr(self.m_scales),
                                                         _ptr(self.v_scales), lr, b1, b2, eps, wd, gscale, _ptr(dev), self.step_dev.data_ptr(), self._ticket.data_ptr(), self.seed, _s())
         if rc != 0:
             raise RuntimeError(f"adamw_many failed (code {rc})")

@@ -20,7 +20,7 @@ struct AdamTensor {
 enum { ADAM_DECAY = 1, ADAM_P_F32 = 2, ADAM_G_F32 = 4, ADAM_WORDS = 8 };      // WORDS: every address on a boundary of eight elements
 
 struct AdamArgs {
-  const AdamTensor* tensors; int count; long long blocks;
+  const AdamTensor* tensors; const int* owner; long long blocks;      // owner: the tensor of each block
   void *m, *v; uint8_t *ms, *vs;
   float lr, b1, c1, b2, c2, eps, wd, lb1, lb2;      // c: 1 - b; lb: logarithms
   float gscale; const float* gscale_dev;
@@ -108,7 +108,7 @@ __device__ __forceinline__ void round_moments(const f32x2 (&m2)[4], const f32x2 
 struct AdamNow {
   bf16* p; float* master; const void* g;                   // p: null if the parameters are the masters
   long long n, first, end;                                 // elements; its first block, that of the next tensor
-  int at, flags;
+  int flags;
 };
 // N words of 4 bytes from N * 4 bytes' boundary on.  Eight of them in one access of 32 bytes: as two of 16 a warp would touch every sector twice.
 template <int N> __device__ __forceinline__ void load_words(const void* p, uint32_t (&w)[N]) {
@@ -123,13 +123,12 @@ template <int N> __device__ __forceinline__ void store_words(void* p, const uint
   else if constexpr (N == 4) *static_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
   else asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");
 }
-__device__ __forceinline__ void adam_find(const AdamArgs& a, long long block, AdamNow& c) {      // the last tensor that begins at or before the block, from c.at on
-  int lo = c.at, hi = a.count;
-  while (hi - lo > 1) { const int mid = (lo + hi) / 2; (a.tensors[mid].block <= block ? lo : hi) = mid; }
-  const AdamTensor& q = a.tensors[lo];
-  c.at = lo; c.flags = q.flags; c.g = q.g; c.n = q.n; c.first = q.block;
+// The tensor of a block.  (By bisection it took eight loads, each waiting for the one before, at almost every block of a thread: a grid is some tensors wide.)
+__device__ __forceinline__ void adam_find(const AdamArgs& a, long long block, AdamNow& c) {
+  const AdamTensor& q = a.tensors[a.owner[block]];
+  c.flags = q.flags; c.g = q.g; c.n = q.n; c.first = q.block;
   c.p = q.flags & ADAM_P_F32 ? nullptr : static_cast<bf16*>(q.p); c.master = q.flags & ADAM_P_F32 ? static_cast<float*>(q.p) : q.master;
-  c.end = lo + 1 < a.count ? a.tensors[lo + 1].block : a.blocks;
+  c.end = q.block + (q.n + 127) / 128;
 }
 // The root of v: in 8 bits the approximate one (2^-23; what it is rounded to has 2^-4), in which v below 2^-126 counts as zero
 template <bool BITS8> __device__ __forceinline__ float adam_root(float v) {
@@ -140,17 +139,13 @@ template <bool BITS8> __device__ __forceinline__ float adam_root(float v) {
 __device__ __forceinline__ float div_approx(float x, float y) { float r; asm("div.approx.ftz.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(y)); return r; }
 
 // What the step is, for every thread of a block.
+// (Every thread computes it for itself while its first loads are under way: through shared memory they would wait for a barrier, a microsecond of a small step's ten.)
 struct AdamStep {
   float rc2, lr1, gscale; uint32_t key;
   __device__ __forceinline__ AdamStep(const AdamArgs& a) {
-    __shared__ float s_c[2];
     const int t = *(volatile int*)a.step + 1;
-    if (threadIdx.x == 0) {
-      s_c[0] = 1.f / -expm1f((float)t * a.lb1);             // 1 - b^t without cancellation
-      s_c[1] = 1.f / sqrtf(-expm1f((float)t * a.lb2));
-    }
-    __syncthreads();
-    rc2 = s_c[1]; lr1 = a.lr * s_c[0];
+    lr1 = a.lr / -expm1f((float)t * a.lb1);                 // 1 - b^t without cancellation
+    rc2 = 1.f / sqrtf(-expm1f((float)t * a.lb2));
     gscale = a.gscale_dev ? a.gscale * *a.gscale_dev : a.gscale;
     key = a.seed + (uint32_t)t * 0x9E3779B9u;
   }
@@ -206,21 +201,22 @@ template <int E> __device__ __forceinline__ void store_weights(float* master, bf
 }
 __device__ __forceinline__ const void* gradients(const AdamNow& c, long long i) { return static_cast<const char*>(c.g) + i * (c.flags & ADAM_G_F32 ? 4 : 2); }
 
-// Moments in fp32: a lane has four elements of a block, a warp the block.  Bound by memory: 28 bytes an element (bf16 parameters and gradients).
-__global__ void __launch_bounds__(256, 5) adamw_many_kernel(const AdamArgs a) {
-  constexpr int E = 4;
+// Moments in fp32: a lane has eight elements, sixteen lanes a block.  Bound by memory: 28 bytes an element (bf16 parameters and gradients, masters).  GPT-2 medium's 355 M parameters: 1570 us, 6.3 TB/s; with four
+// elements a lane and 40 warps to an SM in place of 24 it took 1820, with the next block's lines prefetched 1690.
+__global__ void __launch_bounds__(256, 3) adamw_many_kernel(const AdamArgs a) {
+  constexpr int E = 8;
   pdl_begin();
   const AdamStep step(a);
-  const int l = threadIdx.x & 31;
-  const long long stride = gridDim.x * 8ll;
-  AdamNow now = {nullptr, nullptr, nullptr, 0, 0, -1, 0, 0};
-  for (long long block = blockIdx.x * 8ll + (threadIdx.x >> 5); block < a.blocks; block += stride) {
+  const int l = threadIdx.x & 15;
+  const long long stride = gridDim.x * 16ll;
+  AdamNow now = {nullptr, nullptr, nullptr, 0, 0, -1, 0};
+  for (long long block = blockIdx.x * 16ll + (threadIdx.x >> 4); block < a.blocks; block += stride) {
     if (block >= now.end) adam_find(a, block, now);
     const long long i = (block - now.first) * 128 + l * E, s = block * 128 + l * E;
     const int left = (int)min((long long)E, now.n - i);    // elements of this lane (not positive: none)
     const bool words = (now.flags & ADAM_WORDS) && left == E;
     uint32_t gw[E], w[E];
-    f32x2 m[2], v[2], root[2];
+    f32x2 m[4], v[4], root[4];
     load_words(static_cast<const float*>(a.m) + s, reinterpret_cast<uint32_t (&)[E]>(m));
     load_words(static_cast<const float*>(a.v) + s, reinterpret_cast<uint32_t (&)[E]>(v));
     if (words) {
@@ -235,14 +231,15 @@ __global__ void __launch_bounds__(256, 5) adamw_many_kernel(const AdamArgs a) {
   AdamStep::done(a);
 }
 
-// Moments in 8 bits: a lane has eight elements, sixteen lanes a block, a warp two blocks.  16 bytes an element.
+// Moments in 8 bits: a lane has eight elements, sixteen lanes a block, a warp two blocks.  16 bytes an element (868 us of memory for GPT-2 medium) and about as much arithmetic: two roundings, a root and a division each.
+// 1115 us there, 5.1 TB/s; without the prefetch of the next block's lines 1245, with 16 warps to an SM in place of 24 1395.
 __global__ void __launch_bounds__(256, 3) adamw_many8_kernel(const AdamArgs a) {
   constexpr int E = 8;
   pdl_begin();
   const AdamStep step(a);
   const int l = threadIdx.x & 15, second = threadIdx.x >> 4 & 1;
   const long long stride = gridDim.x * 16ll;
-  AdamNow now = {nullptr, nullptr, nullptr, 0, 0, -1, 0, 0};
+  AdamNow now = {nullptr, nullptr, nullptr, 0, 0, -1, 0};
   for (long long block = blockIdx.x * 16ll + (threadIdx.x >> 4); block - second < a.blocks; block += stride) {
     const bool there = block < a.blocks;                    // the first half of a warp may have the last block
     if (there && block >= now.end) adam_find(a, block, now);
@@ -302,16 +299,16 @@ using namespace piccl_ops;
 
 extern "C" {
 
-// tensors: device array of `count` records in the order of their blocks, which follow each other and cover [0, blocks); m, v: blocks * 128 elements (fp32, or bytes with a byte of scale for each
+// tensors: device array of records in the order of their blocks, which follow each other and cover [0, blocks), none of them empty; owner: device ints, the record of each block; m, v: blocks * 128 elements (fp32, or bytes with a byte of scale for each
 // block); step: device int, steps done so far, advanced by the launch; ticket: device int that holds zero.  gscale_dev: null, or a device float that multiplies gscale.
-int piccl_ops_adamw_many(const void* tensors, int count, long long blocks, int bits8, void* m, void* v, void* ms, void* vs, float lr, double b1, double b2, float eps, float wd, float gscale,
+int piccl_ops_adamw_many(const void* tensors, const int* owner, long long blocks, int bits8, void* m, void* v, void* ms, void* vs, float lr, double b1, double b2, float eps, float wd, float gscale,
                          const float* gscale_dev, int* step, unsigned* ticket, unsigned seed, void* stream) {
-  if (count < 0 || blocks < 0 || !(b1 >= 0 && b1 < 1) || !(b2 >= 0 && b2 < 1)) return -1;
-  if ((blocks && (!tensors || !m || !v || (bits8 && (!ms || !vs)))) || !step || !ticket) return -2;
-  if ((reinterpret_cast<uintptr_t>(m) | reinterpret_cast<uintptr_t>(v)) & 15) return -2;
-  AdamArgs a{static_cast<const AdamTensor*>(tensors), count, blocks, m, v, (uint8_t*)ms, (uint8_t*)vs, lr, (float)b1, (float)(1 - b1), (float)b2, (float)(1 - b2), eps, wd, (float)log(b1), (float)log(b2),
+  if (blocks < 0 || !(b1 >= 0 && b1 < 1) || !(b2 >= 0 && b2 < 1)) return -1;
+  if ((blocks && (!tensors || !owner || !m || !v || (bits8 && (!ms || !vs)))) || !step || !ticket) return -2;
+  if ((reinterpret_cast<uintptr_t>(m) | reinterpret_cast<uintptr_t>(v)) & 31) return -2;      // the kernel's accesses of 32 bytes
+  AdamArgs a{static_cast<const AdamTensor*>(tensors), owner, blocks, m, v, (uint8_t*)ms, (uint8_t*)vs, lr, (float)b1, (float)(1 - b1), (float)b2, (float)(1 - b2), eps, wd, (float)log(b1), (float)log(b2),
              gscale, gscale_dev, step, ticket, seed};
-  const long long want = bits8 ? (blocks + 15) / 16 : (blocks + 7) / 8, most = 148 * (bits8 ? 3 : 5);
+  const long long want = (blocks + 15) / 16, most = 148 * 3;
   const dim3 grid((unsigned)(want < 1 ? 1 : want < most ? want : most));
   const cudaError_t e = launch_pdl(bits8 ? adamw_many8_kernel : adamw_many_kernel, grid, 256, 0, (cudaStream_t)stream, a);
   return e == cudaSuccess ? 0 : (int)e;

@@ -26,7 +26,7 @@ int piccl_ops_attn_rows(int S);
 int piccl_ops_attn_fwd(const void* qkv, void* out, float* lse, int B, int S, int H, void* stream);
 int piccl_ops_attn_parts(int B, int S);
 int piccl_ops_attn_bwd(const void* qkv, const void* out, const void* dout, const float* lse, float* scratch, void* dqkv, float* part, int B, int S, int H, void* stream);
-int piccl_ops_adamw_many(const void* tensors, int count, long long blocks, int bits8, void* m, void* v, void* ms, void* vs, float lr, double b1, double b2, float eps, float wd, float gscale,
+int piccl_ops_adamw_many(const void* tensors, const int* owner, long long blocks, int bits8, void* m, void* v, void* ms, void* vs, float lr, double b1, double b2, float eps, float wd, float gscale,
                          const float* gscale_dev, int* step, unsigned* ticket, unsigned seed, void* stream);
 int piccl_ops_fp8_quantize(const void* x, int fp32, long long R, long long C, long long stride, void* q, void* qs, void* t, void* ts, int square, void* stream);
 int piccl_ops_fp8_gemm(const void* a, const void* sa, const void* b, const void* sb, const void* bias, void* out, int f32, int M, int N, long long K, int force_tn, void* stream);

@@ -72,6 +72,6 @@ def test_adamw_refuses():
     step = N.ops_lib().piccl_ops_adamw_many
     step.argtypes = _STEP
     good = 4096
-    ok = [good, 1, 1, 1, good, good, good, good, 1e-3, 0.9, 0.95, 1e-8, 0.1, 1.0, 0, good, good, 0, 0]
-    for at, bad, rc in ((0, 0, -2), (1, -1, -1), (2, -1, -1), (4, 0, -2), (4, good + 8, -2), (5, good + 4, -2), (6, 0, -2), (7, 0, -2), (9, 1.0, -1), (9, -0.1, -1), (10, 1.5, -1), (15, 0, -2), (16, 0, -2)):
+    ok = [good, good, 1, 1, good, good, good, good, 1e-3, 0.9, 0.95, 1e-8, 0.1, 1.0, 0, good, good, 0, 0]
+    for at, bad, rc in ((0, 0, -2), (1, 0, -2), (2, -1, -1), (4, 0, -2), (4, good + 8, -2), (5, good + 4, -2), (6, 0, -2), (7, 0, -2), (9, 1.0, -1), (9, -0.1, -1), (10, 1.5, -1), (15, 0, -2), (16, 0, -2)):
         assert step(*[bad if i == at else x for i, x in enumerate(ok)]) == rc, (at, bad)
