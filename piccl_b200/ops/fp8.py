@@ -1,4 +1,4 @@
-"""Linear layers in 8 bits: the quantiser and the products of src/ops/fp8_quant.cu and fp8_gemm.cu.
+"""Linear layers in 8 bits: the quantiser and the products of src/ops/fp8_quant.cu, fp8_gemm.cu and, for few rows, fp8_few.cu.
 
 A matrix in 8 bits (`Fp8`) is e4m3 values, rows filled with zeros to a multiple of 128, and one power of two for each block of 128
 values of a row: byte e, 1 to 254, stands for 2^(e - 127), the smallest for which the block's largest finite magnitude is at most 448.  Values that
@@ -12,13 +12,13 @@ dimensions is kept twice, the second time transposed; `square` gives both copies
     fp8.linear_bwd(dy, xt, w8t, dx, dw)                      # dx = dy w, dw = dy^T x
 
 Sums are fp32 in the tensor cores; results are rounded once.  Calls launch on the current stream of their tensors' device, take workspace from PyTorch's
-allocator, and can be captured.  Empty results are left alone; a sum over nothing is zero (or the bias).
+allocator, and can be captured.  Results overlap neither operands nor each other.  Empty results are left alone; a sum over nothing is zero (or the bias).
 """
 from __future__ import annotations
 
 import ctypes as C
 from contextlib import nullcontext
-from typing import NamedTuple, Optional
+from typing import NamedTuple, Optional, Sequence
 
 import torch
 
@@ -93,6 +93,14 @@ def _check_matrix(x: torch.Tensor, name: str, dtypes, contiguous: bool) -> None:
         raise ValueError(f"{name}: tensors of one CUDA device wanted")
 
 
+def _check_apart(name: str, written: Sequence[Optional[torch.Tensor]], read: Sequence[Optional[torch.Tensor]]) -> None:
+    """What is written shares no bytes with what is read, nor with what else is written: blocks of a launch read operands while others write."""
+    bytes_of = lambda t: (t.data_ptr(), t.data_ptr() + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size())  # noqa: E731
+    w, r = ([bytes_of(t) for t in ts if t is not None and t.numel()] for ts in (written, read))
+    if any(a[0] < b[1] and b[0] < a[1] for i, a in enumerate(w) for b in w[i + 1:] + r):
+        raise ValueError(f"{name}: operands and results that overlap")
+
+
 def _done(rc: int, what: str) -> None:
     if rc != 0:
         raise RuntimeError(f"{what} failed (code {rc})")
@@ -115,6 +123,7 @@ def quantize(x: torch.Tensor, out: Optional[Fp8], transposed: Optional[Fp8] = No
             _check_fp8(a, "quantize", x.device)
             if tuple(a.values.shape) != (rows, (cols + 127) // 128 * 128):
                 raise ValueError(f"quantize: room for {rows} x {cols} wanted, got {tuple(a.values.shape)}")
+    _check_apart("quantize", [*(out or ()), *(transposed or ())], [x])
     if R == 0 or Cc == 0:
         for a in (out, transposed):
             if a is not None:
@@ -144,6 +153,7 @@ def product(a: Fp8, b: Fp8, out: torch.Tensor, bias: Optional[torch.Tensor] = No
         return out
     _check_fp8(a, "product", out.device)
     _check_product(tuple(a.values.shape), b, out, bias)
+    _check_apart("product", [out], [*a, *b, bias])
     (M, K), Nn = a.values.shape, b.values.shape[0]
     if M == 0 or Nn == 0:
         return out
@@ -163,6 +173,7 @@ def linear(x: torch.Tensor, w: Fp8, out: torch.Tensor, bias: Optional[torch.Tens
         return out
     _check_matrix(x, "linear", (torch.bfloat16, torch.float32), False)
     M, K = x.shape
+    _check_apart("linear", [out, *(keep or ())], [x, *w, bias])
     if w.values.dim() != 2 or w.values.shape[1] != (K + 127) // 128 * 128:
         raise ValueError(f"linear: weights of {K} columns wanted, got {tuple(w.values.shape)}")
     if keep is None and M and K and M <= 64 and not _native("piccl_ops_fp8_linear_scratch", _SCRATCH)(x.data_ptr(), x.dtype == torch.float32, x.stride(0) if M > 1 else K, M, w.values.shape[0], K, False):
@@ -194,6 +205,7 @@ def linear_bwd(dy: torch.Tensor, xt: Optional[Fp8], wt: Optional[Fp8], dx: Optio
     if (dx is not None and wt is None) or (dw is not None and xt is None):
         raise ValueError("linear_bwd: dx takes the transposed weights, dw the input along the tokens")
     M, Nn = dy.shape
+    _check_apart("linear_bwd", [dx, dw], [dy, *(xt or ()), *(wt or ())])
     for a, n in ((wt if dx is not None else None, Nn), (xt if dw is not None else None, M)):
         if a is not None and (a.values.dim() != 2 or a.values.shape[1] != (n + 127) // 128 * 128):
             raise ValueError(f"linear_bwd: {n} columns wanted, got {tuple(a.values.shape)}")

@@ -22,16 +22,21 @@ __device__ __forceinline__ void mma_e4m3(float (&c)[4], uint32_t a0, uint32_t a1
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// acc += what a block of 128 k gives: rows g and g + 8 of 16 rows of B (two chunks of 64 k, 16 bytes each), row g of 8 rows of A; f: powers of the rows of B, x: of rows 2 t and 2 t + 1 of A
-__device__ __forceinline__ void add_block(float (&acc)[4], const uint4 (&w)[2][2], const uint4 (&b)[2], float f0, float f1, float x0, float x1) {
+// acc += what a block of 128 k gives: rows g and g + 8 of 16 rows of B (two chunks of 64 k, 16 bytes each), row g of 8 rows of A; f: bytes of the scales of the rows of B, x: of rows 2 t and 2 t + 1 of A, all moved to bit 22.
+// The product of two scales has twice the range of fp32, and one may be far above 1 where the other is far below, so half of their sum of exponents is multiplied by first, the rest after it: each partial
+// result is then between 2^-145 and the last one.
+__device__ __forceinline__ void add_block(float (&acc)[4], const uint4 (&w)[2][2], const uint4 (&b)[2], uint32_t f0, uint32_t f1, uint32_t x0, uint32_t x1) {
   float c[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int k = 0; k < 2; k++) {
     mma_e4m3(c, w[0][k].x, w[1][k].x, w[0][k].y, w[1][k].y, b[k].x, b[k].y);
     mma_e4m3(c, w[0][k].z, w[1][k].z, w[0][k].w, w[1][k].w, b[k].z, b[k].w);
   }
-  acc[0] = fmaf(c[0] * f0, x0, acc[0]); acc[1] = fmaf(c[1] * f0, x1, acc[1]);
-  acc[2] = fmaf(c[2] * f1, x0, acc[2]); acc[3] = fmaf(c[3] * f1, x1, acc[3]);
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    const uint32_t both = (i < 2 ? f0 : f1) + (i & 1 ? x1 : x0), half = both & 0x7f800000u;
+    acc[i] = fmaf(c[i] * __uint_as_float(half), __uint_as_float(2 * both - half), acc[i]);
+  }
 }
 // sums: [8 warps][8 T][16 R + 1]
 template <int R, int T> __device__ __forceinline__ void put_sums(float* sums, const float (&acc)[R][T][4], int warp, int g, int t) {
@@ -62,12 +67,12 @@ __device__ __forceinline__ void prefetch_rows(const FewArgs& a, int row0, int ro
   }
 }
 
-// A in shared memory: 8 T rows of kb * 128 bytes, 16-byte pieces of a block moved by the row so that eight lanes beside each other, four pieces of two rows, meet in no bank, and the scales as
-// powers of two in fp32 for each block and row.
+// A in shared memory: 8 T rows of kb * 128 bytes, 16-byte pieces of a block moved by the row so that eight lanes beside each other, four pieces of two rows, meet in no bank, and the scales'
+// bytes, moved to bit 22, for each block and row.
 struct FewA {
-  uint4* x; float* f; int kb;
+  uint4* x; uint32_t* f; int kb;
   __device__ __forceinline__ uint4* piece(int row, int block, int i) const { return x + ((size_t)row * kb + block) * 8 + (i ^ (row & 1) << 2 ^ (row >> 1 & 3)); }
-  __device__ __forceinline__ float* power(int row, int block, int rows) const { return f + (size_t)block * rows + row; }
+  __device__ __forceinline__ uint32_t* scale(int row, int block, int rows) const { return f + (size_t)block * rows + row; }
 };
 
 // R: groups of 16 rows of B, T: groups of 8 rows of A, D: blocks of B that a warp has under way
@@ -75,7 +80,7 @@ template <int R, int T, int D, typename O>
 __global__ void __launch_bounds__(256, R * T <= 2 ? 2 : 1) fp8_few_kernel(const FewArgs a) {
   constexpr int ROWS = 16 * R, COLS = 8 * T;
   extern __shared__ __align__(16) uint4 few_smem[];
-  const FewA A{few_smem, reinterpret_cast<float*>(few_smem + (size_t)COLS * a.kb * 8), a.kb};
+  const FewA A{few_smem, reinterpret_cast<uint32_t*>(few_smem + (size_t)COLS * a.kb * 8), a.kb};
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int row0 = blockIdx.x * ROWS;
   const long long pitch = 128ll * a.kb;
@@ -125,7 +130,7 @@ __global__ void __launch_bounds__(256, R * T <= 2 ? 2 : 1) fp8_few_kernel(const 
         const uint2 lo = pack_row(v[u][0], f, odd), hi = pack_row(v[u][1], f, odd);
         if (i < items) {
           *A.piece(m, kb, l8) = make_uint4(lo.x, lo.y, hi.x, hi.y);
-          if (l8 == 0) *A.power(m, kb, COLS) = scale_value(byte);
+          if (l8 == 0) *A.scale(m, kb, COLS) = byte << 22;
         }
       }
     }
@@ -149,11 +154,9 @@ __global__ void __launch_bounds__(256, R * T <= 2 ? 2 : 1) fp8_few_kernel(const 
         uint4 b[2];                                        // row 8 n + g of A
 #pragma unroll
         for (int k = 0; k < 2; k++) b[k] = *A.piece(8 * n + g, kb, 4 * k + t);
-        const float2 fx = *reinterpret_cast<const float2*>(A.power(8 * n + 2 * t, kb, COLS));
+        const uint2 fx = *reinterpret_cast<const uint2*>(A.scale(8 * n + 2 * t, kb, COLS));
 #pragma unroll
-        for (int r = 0; r < R; r++) {
-          add_block(acc[r][n], p.w[r], b, scale_value(p.s[r][0]), scale_value(p.s[r][1]), fx.x, fx.y);
-        }
+        for (int r = 0; r < R; r++) add_block(acc[r][n], p.w[r], b, p.s[r][0] << 22, p.s[r][1] << 22, fx.x, fx.y);
       }
       if (kb + 8 * D < a.kb) load(part[d], kb + 8 * D);
     }
@@ -213,7 +216,7 @@ __global__ void __launch_bounds__(256, 1) fp8_fragments_kernel(const FewArgs a) 
 #pragma unroll
       for (int n = 0; n < T; n++)
 #pragma unroll
-        for (int r = 0; r < R; r++) add_block(acc[r][n], p.w[r], p.b[n], scale_value(p.s[r][0]), scale_value(p.s[r][1]), scale_value(p.f[n][0]), scale_value(p.f[n][1]));
+        for (int r = 0; r < R; r++) add_block(acc[r][n], p.w[r], p.b[n], p.s[r][0] << 22, p.s[r][1] << 22, p.f[n][0] << 22, p.f[n][1] << 22);
       if (kb + 8 * D < a.kb) load(part[d], kb + 8 * D);
     }
   }

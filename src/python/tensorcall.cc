@@ -4,6 +4,7 @@
 // scratch and the conversion of arguments.  Each function here returns the number of launches, or 0 if anything about its arguments is not as it has to be (or nothing is to be launched): the
 // Python function then looks at them itself and says what is wrong.
 #include <Python.h>
+#include <initializer_list>
 #include <new>
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
@@ -42,6 +43,23 @@ bool bias_fits(PyObject* o, const at::Tensor& out, const at::Tensor*& bias) {
   bias = tensor(o);
   return bias && bias->scalar_type() == at::kBFloat16 && bias->dim() == 1 && bias->size(0) == out.size(1) && bias->is_contiguous() && bias->device() == out.device();
 }
+// What is written shares no bytes with what is read, nor with what else is written (the first `written` of them); null pointers are passed over
+bool apart(std::initializer_list<const at::Tensor*> all, size_t written) {
+  struct Range { uintptr_t lo, hi; } r[10];
+  size_t n = 0;
+  for (const at::Tensor* t : all) {
+    Range& q = r[n++];
+    q = {0, 0};
+    if (!t || t->numel() == 0) continue;
+    long long last = 0;
+    for (int64_t d = 0; d < t->dim(); d++) last += (t->size(d) - 1) * t->stride(d);
+    q.lo = reinterpret_cast<uintptr_t>(t->data_ptr()); q.hi = q.lo + (last + 1) * t->element_size();
+  }
+  for (size_t i = 0; i < written; i++)
+    for (size_t j = i + 1; j < n; j++)
+      if (r[i].lo < r[j].hi && r[j].lo < r[i].hi) return false;
+  return true;
+}
 void* ptr(const at::Tensor* t) { return t ? t->data_ptr() : nullptr; }
 void* stream() { return at::cuda::getCurrentCUDAStream().stream(); }
 
@@ -72,6 +90,7 @@ PyObject* quantize(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (!matrix(x, false) || (a[1] == Py_None && a[2] == Py_None)) return no();
     if (a[1] != Py_None && !(eight(a[1], x->device(), q) && has_room(q, x->size(0), x->size(1)))) return no();
     if (a[2] != Py_None && !(eight(a[2], x->device(), t) && has_room(t, x->size(1), x->size(0)))) return no();
+    if (!apart({q.v, q.s, t.v, t.s, x}, 4)) return no();
     const int square = PyObject_IsTrue(a[3]);
     if (square < 0) return nullptr;
     const c10::cuda::CUDAGuard guard(x->device());
@@ -86,6 +105,7 @@ PyObject* product(PyObject*, PyObject* const* a, Py_ssize_t n) {
     Eight x, w;
     if (!matrix(out, true) || !eight(a[0], out->device(), x) || !eight(a[1], out->device(), w) || !bias_fits(a[3], *out, bias)) return no();
     if (x.v->size(1) != w.v->size(1) || x.v->size(1) == 0 || x.v->size(0) != out->size(0) || w.v->size(0) != out->size(1)) return no();
+    if (!apart({out, x.v, x.s, w.v, w.s, bias}, 1)) return no();
     const c10::cuda::CUDAGuard guard(out->device());
     return answer(piccl_ops_fp8_gemm(ptr(x.v), ptr(x.s), ptr(w.v), ptr(w.s), ptr(bias), out->data_ptr(), out->scalar_type() == at::kFloat, (int)out->size(0), (int)out->size(1), x.v->size(1), 0, stream()), 1,
                   "fp8 product");
@@ -99,6 +119,7 @@ PyObject* linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
     Eight w, keep;
     if (!matrix(x, false) || !matrix(out, true) || out->device() != x->device() || !eight(a[1], x->device(), w) || !has_room(w, out->size(1), x->size(1)) || out->size(0) != x->size(0)) return no();
     if (!bias_fits(a[3], *out, bias) || (a[4] != Py_None && !(eight(a[4], x->device(), keep) && has_room(keep, x->size(1), x->size(0))))) return no();
+    if (!apart({out, keep.v, keep.s, x, w.v, w.s, bias}, 3)) return no();
     const c10::cuda::CUDAGuard guard(x->device());
     const int M = (int)x->size(0), fp32 = x->scalar_type() == at::kFloat, f32 = out->scalar_type() == at::kFloat;
     const long long K = x->size(1), stride = row_stride(*x);
@@ -128,6 +149,7 @@ PyObject* linear_bwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
       dw = tensor(a[4]);
       if (!matrix(dw, true) || dw->device() != dy->device() || !eight(a[1], dy->device(), xt) || !has_room(xt, dw->size(1), M) || dw->size(0) != N) return no();
     }
+    if (!apart({dx, dw, dy, xt.v, xt.s, wt.v, wt.s}, 2)) return no();
     const c10::cuda::CUDAGuard guard(dy->device());
     const Scratch q(dx ? M : 0, N), t(dw ? N : 0, M);
     int rc = piccl_ops_fp8_quantize(dy->data_ptr(), dy->scalar_type() == at::kFloat, M, N, row_stride(*dy), dx ? q.v : nullptr, dx ? q.s : nullptr, dw ? t.v : nullptr, dw ? t.s : nullptr, 0, stream());

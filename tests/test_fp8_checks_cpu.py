@@ -46,6 +46,16 @@ def test_products_refuse():
         fp8.linear_bwd(torch.zeros(4, 8, dtype=BF), None, None, None, torch.zeros(8, 128))
 
 
+def test_what_overlaps():
+    from piccl_b200.ops.fp8 import _check_apart
+    x = torch.zeros(8, 16)
+    _check_apart("f", [x[:4], None], [x[4:], x[:0]])
+    _check_apart("f", [x[0]], [x[1:, :3], x[0, :0]])
+    for written, read in (([x[:4]], [x[3:]]), ([x[:4], x[3:5]], []), ([x[2]], [x[:, :1]]), ([x], [None, x.view(torch.int16)[5:6]])):
+        with pytest.raises(ValueError, match="overlap"):
+            _check_apart("f", written, read)
+
+
 def test_native_entries_refuse_before_they_touch_an_address():
     from piccl_b200 import _native as N
     from piccl_b200.ops import fp8
@@ -73,5 +83,5 @@ def test_adamw_refuses():
     step.argtypes = _STEP
     good = 4096
     ok = [good, good, 1, 1, good, good, good, good, 1e-3, 0.9, 0.95, 1e-8, 0.1, 1.0, 0, good, good, 0, 0]
-    for at, bad, rc in ((0, 0, -2), (1, 0, -2), (2, -1, -1), (4, 0, -2), (4, good + 8, -2), (5, good + 4, -2), (6, 0, -2), (7, 0, -2), (9, 1.0, -1), (9, -0.1, -1), (10, 1.5, -1), (15, 0, -2), (16, 0, -2)):
+    for at, bad, rc in ((0, 0, -2), (1, 0, -2), (2, -1, -1), (4, 0, -2), (4, good + 8, -2), (4, good + 16, -2), (5, good + 4, -2), (6, 0, -2), (7, 0, -2), (9, 1.0, -1), (9, -0.1, -1), (10, 1.5, -1), (15, 0, -2), (16, 0, -2)):
         assert step(*[bad if i == at else x for i, x in enumerate(ok)]) == rc, (at, bad)

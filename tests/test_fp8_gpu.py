@@ -184,6 +184,25 @@ def test_the_ends_of_the_range(scale):
         _same(t, x.t(), square)
 
 
+@pytest.mark.parametrize("M,N,K", [(1, 64, 256), (8, 5000, 264), (16, 256, 512), (24, 128, 1024), (200, 256, 1280)])
+@pytest.mark.parametrize("up,down", [(120, -30), (-30, 120), (110, -118), (-118, 110), (-60, -50)])
+def test_products_of_large_and_small_scales(M, N, K, up, down):
+    """The scale of one operand may be far above 1 where the other's is far below: the bound is that of any product."""
+    from piccl_b200.ops import fp8
+    x, w = _randn(M, K, seed=1, scale=2.0 ** up), _randn(N, K, seed=2, scale=2.0 ** down)
+    q, w8 = fp8.empty(M, K), fp8.empty(N, K)
+    fp8.quantize(x, q)
+    fp8.quantize(w, w8)
+    a, b = ((t.values.double() * torch.exp2(fp8.exponents(t).double() - 127).repeat_interleave(128, 1)) for t in (q, w8))
+    want, size = a @ b.t(), a.abs() @ b.t().abs()
+    for dtype, eps in ((torch.bfloat16, EPS16), (torch.float32, EPS32)):
+        y, z = (torch.empty(M, N, dtype=dtype, device="cuda") for _ in range(2))
+        fp8.linear(x, w8, y)
+        fp8.product(q, w8, z)
+        for got in (y, z):
+            assert bool(((got.double() - want).abs() <= 2 * EPS32 * (K / 32 + 10) * size + eps * want.abs()).all())
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("offset,extra", [(0, 0), (1, 0), (0, 3), (8, 8), (3, 16)])
 def test_strided_rows_at_any_address(dtype, offset, extra):
@@ -283,6 +302,27 @@ def test_refusals_on_the_gpu():
                  lambda: fp8.linear_bwd(y, None, w, torch.empty(4, 128, dtype=torch.bfloat16, device="cuda"), None)):
         with pytest.raises(ValueError):
             call()
+
+
+def test_results_that_overlap_operands_are_refused():
+    """In place a block of a launch would write what another has yet to read."""
+    from piccl_b200.ops import fp8
+    x, w, wt = _randn(4, 128), fp8.empty(128, 128), fp8.empty(128, 128)
+    fp8.quantize(_randn(128, 128), w, transposed=wt, square=True)
+    q, xt, y, dw = fp8.empty(4, 128), fp8.empty(128, 4), torch.zeros_like(x), torch.empty(128, 128, dtype=torch.bfloat16, device="cuda")
+    fp8.quantize(x, q, transposed=xt)
+    row = torch.zeros(1, 128, dtype=torch.bfloat16, device="cuda")
+    q1 = fp8.empty(1, 128)
+    fp8.quantize(row, q1)
+    inside = xt.values.view(torch.bfloat16)[:8].view(4, 128)          # room within xt
+    assert inside.data_ptr() == xt.values.data_ptr()
+    before = x.clone()
+    for call in (lambda: fp8.linear(x, w, x), lambda: fp8.linear(row, w, row), lambda: fp8.product(q1, w, row, bias=row[0]), lambda: fp8.product(q, w, w.values.view(torch.bfloat16)[:8].view(4, 128)),
+                 lambda: fp8.quantize(x, q, transposed=fp8.Fp8(xt.values, q.scales)), lambda: fp8.quantize(x, fp8.Fp8(x.view(fp8.E4M3)[:2].view(4, 128), q.scales)),
+                 lambda: fp8.linear_bwd(y, xt, wt, y, dw), lambda: fp8.linear_bwd(y, xt, wt, inside, dw), lambda: fp8.linear_bwd(y, xt, wt, dw[:4], dw)):
+        with pytest.raises(ValueError, match="overlap"):
+            call()
+    assert torch.equal(x, before)
 
 
 def test_calls_close_on_each_other_streams_and_graphs():
