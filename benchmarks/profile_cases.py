@@ -14,6 +14,8 @@
     python benchmarks/profile_cases.py ag_gemm   # fused all-gather -> GEMM, 2 virtual ranks, 4096 x 2048 x 4096
     python benchmarks/profile_cases.py attention # causal attention forward and backward, 8 x 1024 tokens, 16 heads of 64 columns
     python benchmarks/profile_cases.py elementwise  # AdamW on 128 Mi parameters, bias + GELU forward / backward on 8192 x 4096, embedding 8192 x 1024, column sum
+    python benchmarks/profile_cases.py fp8       # 8-bit layers: quantiser 8192 x 4096 both ways, products 8192 x 4096 x 1024 and of 1 and 24 rows
+    python benchmarks/profile_cases.py adamw_many   # AdamW over 24 tensors of 4 Mi parameters, moments in fp32 and in 8 bits
 
 Typical capture (after the same command has exited 0 without ncu):
     ncu --set full --clock-control none -k regex:<kernel> -s 2 -c 2 -o <name> python benchmarks/profile_cases.py <case>
@@ -201,7 +203,36 @@ def case_ce():
     torch.cuda.synchronize()
 
 
+def case_fp8():
+    from piccl_b200.ops import fp8
+    x, x1 = torch.randn(8192, 4096, device="cuda").bfloat16(), torch.randn(8192, 1024, device="cuda").bfloat16()
+    q, t, w, y = fp8.empty(8192, 4096), fp8.empty(4096, 8192), fp8.empty(4096, 1024), torch.empty(8192, 4096, device="cuda", dtype=torch.bfloat16)
+    fp8.quantize(torch.randn(4096, 1024, device="cuda"), w, square=True)
+    wide, out = fp8.empty(1024, 4096), torch.empty(24, 1024, device="cuda", dtype=torch.bfloat16)
+    fp8.quantize(torch.randn(1024, 4096, device="cuda"), wide)
+    for _ in range(3):
+        fp8.quantize(x, q, transposed=t)
+        fp8.linear(x1, w, y)
+        fp8.linear(x[:1], wide, out[:1])
+        fp8.linear(x[:24], wide, out)
+    torch.cuda.synchronize()
+    assert torch.isfinite(y).all() and torch.isfinite(out).all()
+
+
+def case_adamw_many():
+    from piccl_b200.ops.optimizer import AdamW
+    n, k = 4 << 20, 24
+    masters = [torch.randn(n, device="cuda") for _ in range(k)]
+    params, grads = [w.bfloat16() for w in masters], [torch.randn(n, device="cuda").bfloat16() for _ in range(k)]
+    opts = [AdamW(params, grads, masters, bits=b) for b in (32, 8)]
+    for _ in range(3):
+        for o in opts:
+            o.step(1e-4)
+    torch.cuda.synchronize()
+    assert all(torch.isfinite(w).all() for w in masters)
+
+
 if __name__ == "__main__":
     which = sys.argv[1] if len(sys.argv) > 1 else "exec"
-    {"exec": case_exec, "flow": case_flow, "exec8": lambda: case_exec(8, 8 << 20), "exec_ll": lambda: case_exec(8, 4096, "PRD"), "gemm": case_gemm, "direct": case_direct, "tp": case_tp, "ln": case_ln, "ce": case_ce, "nvls": case_nvls, "llf": case_llf, "ag_gemm": case_ag_gemm, "attention": case_attention, "elementwise": case_elementwise}[which]()
+    {"exec": case_exec, "flow": case_flow, "exec8": lambda: case_exec(8, 8 << 20), "exec_ll": lambda: case_exec(8, 4096, "PRD"), "gemm": case_gemm, "direct": case_direct, "tp": case_tp, "ln": case_ln, "ce": case_ce, "nvls": case_nvls, "llf": case_llf, "ag_gemm": case_ag_gemm, "attention": case_attention, "elementwise": case_elementwise, "fp8": case_fp8, "adamw_many": case_adamw_many}[which]()
     print(f"profile case {which} done")

@@ -62,7 +62,7 @@ __device__ __forceinline__ uint32_t scale_byte_of_root(uint32_t v_bits) {
   return v_bits < 0x00800000u ? 1u : (uint32_t)s;
 }
 __device__ __forceinline__ uint2 e4m3_bytes(const float (&t)[8]) {
-  return make_uint2(e4m3_pair(t[0], t[1]) | e4m3_pair(t[2], t[3]) << 16, e4m3_pair(t[4], t[5]) | e4m3_pair(t[6], t[7]) << 16);
+  return make_uint2(e4m3_four(t[0], t[1], t[2], t[3]), e4m3_four(t[4], t[5], t[6], t[7]));
 }
 // Eight moments and roots of a block, by 16 lanes -> their bytes and the block's two.  All lanes of a warp call it together (votes and shuffles among a part of them cost a barrier each), and both
 // maxima are found side by side: one after the other, each behind its own votes, the latencies of shuffles were a third of the kernel's time.

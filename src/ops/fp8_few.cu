@@ -121,13 +121,12 @@ __global__ void __launch_bounds__(256, R * T <= 2 ? 2 : 1) fp8_few_kernel(const 
         const int i = i0 + 32 * u, m = i / a.kb, kb = i - m * a.kb;
         if (i - (threadIdx.x >> 3 & 3) >= items) break;      // none of the warp's four
         uint32_t top = max(top8(v[u][0]), top8(v[u][1]));
-        const bool odd = __any_sync(0xffffffffu, top >= kInf);
-        if (odd) top = max(finite_top8(v[u][0]), finite_top8(v[u][1]));
+        if (__any_sync(0xffffffffu, top >= kInf)) { top = max(finite_top8(v[u][0]), finite_top8(v[u][1])); no_inf(v[u][0]); no_inf(v[u][1]); }
 #pragma unroll
         for (int o = 4; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
         const uint32_t byte = scale_byte(top);
         const float f = scale_inverse(byte);
-        const uint2 lo = pack_row(v[u][0], f, odd), hi = pack_row(v[u][1], f, odd);
+        const uint2 lo = pack_row(v[u][0], f), hi = pack_row(v[u][1], f);
         if (i < items) {
           *A.piece(m, kb, l8) = make_uint4(lo.x, lo.y, hi.x, hi.y);
           if (l8 == 0) *A.scale(m, kb, COLS) = byte << 22;

@@ -1,5 +1,6 @@
 // bf16 or fp32 matrices -> e4m3 with a power of two for each block of 128 (fp8.cuh), along the rows, along the columns (the transposed copy, which a product
 // over the other dimension takes) or both in one pass over the matrix.  Square: one power of two for each 128 x 128, so that both copies stand for the same values.
+#include <atomic>
 #include "fp8.cuh"
 
 namespace piccl_ops {
@@ -36,14 +37,13 @@ __global__ void __launch_bounds__(256) quant_rows_kernel(const QuantArgs a) {
   load8<T, VEC>(x, c, a.C, v[0]);
   load8<T, VEC>(x, c + 8, a.C, v[1]);
   uint32_t top = max(top8(v[0]), top8(v[1]));
-  const bool odd = __any_sync(0xffffffffu, top >= kInf);
-  if (odd) top = max(finite_top8(v[0]), finite_top8(v[1]));
+  if (__any_sync(0xffffffffu, top >= kInf)) { top = max(finite_top8(v[0]), finite_top8(v[1])); no_inf(v[0]); no_inf(v[1]); }
 #pragma unroll
   for (int o = 4; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
   const uint32_t byte = scale_byte(top);
   const float f = scale_inverse(byte);
   if (c < a.kc) {
-    const uint2 lo = pack_row(v[0], f, odd), hi = pack_row(v[1], f, odd);
+    const uint2 lo = pack_row(v[0], f), hi = pack_row(v[1], f);
     *reinterpret_cast<uint4*>(a.q + row * a.kc + c) = make_uint4(lo.x, lo.y, hi.x, hi.y);
   }
   uint32_t all = byte << (8 * (lane >> 3));
@@ -53,7 +53,8 @@ __global__ void __launch_bounds__(256) quant_rows_kernel(const QuantArgs a) {
 }
 
 // A block has a tile of 128 x 128 in registers as it came, a thread 8 x 8 of it (16 lanes beside each other to a row).  The largest magnitudes of its rows and columns go through shared memory
-// at one barrier; half of the threads then put the rows' together, half the columns'.  (The rows' by shuffles, 32 a thread: 42 us for 8192 x 4096 bf16 both ways.)
+// at one barrier; half of the threads then put the rows' together, half the columns'.  (The rows' by shuffles, 32 a thread: 42 us for
+// 8192 x 4096 bf16 both ways, in place of 26.5.)  Bound by the latencies of loads and barriers at 17 instructions a value, 5.1 TB/s; four blocks to an SM, at 64 registers and a spill of two, take 26.5 us where three take 27.2.
 // Magnitudes of the two kinds: 128 lines of 16 partial maxima, a line's partial i at [i][line], and every [i] moved on by 16 bytes so that threads side by side do not meet in a bank.
 template <typename T> struct Tops {
   static constexpr int PITCH = 128 * sizeof(T) + 16;       // bf16: 16 bits each
@@ -68,7 +69,7 @@ template <typename T> struct Tops {
   }
 };
 template <typename T, bool VEC, bool ROWS, bool COLS, bool SQUARE>
-__global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2) quant_tile_kernel(const QuantArgs a) {
+__global__ void __launch_bounds__(256, sizeof(T) == 2 ? 4 : 2) quant_tile_kernel(const QuantArgs a) {
   constexpr int W = Eight<T>::W, B = sizeof(T) == 2;
   union Shared {
     struct { Tops<T> rows, cols; } tops;
@@ -112,13 +113,11 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2) quant_tile_kernel
     }
   };
   float square = 0.f;
-  bool odd;
   if (SQUARE) {
-    odd = __syncthreads_or(top >= kInf);
-    if (odd) {
+    if (__syncthreads_or(top >= kInf)) {
       top = 0;
 #pragma unroll
-      for (int i = 0; i < 8; i++) top = max(top, finite_top8(v[i]));
+      for (int i = 0; i < 8; i++) { top = max(top, finite_top8(v[i])); no_inf(v[i]); }
     }
     top = __reduce_max_sync(0xffffffffu, top);
     if ((threadIdx.x & 31) == 0) sh.warps[threadIdx.x >> 5] = top;
@@ -137,8 +136,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2) quant_tile_kernel
       if (B) row[i >> 1] = i & 1 ? row[i >> 1] | m : m >> 16;
       else row[i] = m;
     }
-    odd = __syncthreads_or(top >= kInf);
-    if (odd) {
+    if (__syncthreads_or(top >= kInf)) {
 #pragma unroll
       for (int i = 0; i < 8; i++) {
         const uint32_t m = finite_top8(v[i]);
@@ -154,6 +152,8 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2) quant_tile_kernel
           for (int h = 0; h < 8 / W; h++) m[h] = max(m[h], finite_bits(v[i].at(8 / W * e + h)));
         col[e] = B ? m[0] >> 16 | (m[1] & 0xffff0000u) : m[0];
       }
+#pragma unroll
+      for (int i = 0; i < 8; i++) no_inf(v[i]);
     }
 #pragma unroll
     for (int e = 0; e < W; e += 4) {
@@ -173,7 +173,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2) quant_tile_kernel
 #pragma unroll
     for (int i = 0; i < 8; i++) {
       const float f = SQUARE ? square : scale_inverse(((i < 4 ? eight.x : eight.y) >> (8 * (i & 3))) & 255u);
-      if (r0 + i < a.R) *reinterpret_cast<uint2*>(a.q + (r0 + i) * a.kc + c0) = pack_row(v[i], f, odd);
+      if (r0 + i < a.R) *reinterpret_cast<uint2*>(a.q + (r0 + i) * a.kc + c0) = pack_row(v[i], f);
     }
   }
   if (COLS) {
@@ -184,7 +184,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2) quant_tile_kernel
       const float f = SQUARE ? square : scale_inverse(((e < 4 ? eight.x : eight.y) >> (8 * (e & 3))) & 255u);
       float w[8];
 #pragma unroll
-      for (int i = 0; i < 8; i++) { w[i] = v[i].at(e); if (odd) w[i] = nan_of_inf(w[i]); }
+      for (int i = 0; i < 8; i++) w[i] = v[i].at(e);
       *reinterpret_cast<uint2*>(sh.turned + (cg * 8 + e) * 128 + ((rg ^ cg) << 3)) = make_uint2(pack4(w[0], w[1], w[2], w[3], f), pack4(w[4], w[5], w[6], w[7], f));
     }
     __syncthreads();
@@ -197,15 +197,33 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2) quant_tile_kernel
   }
 }
 
+// Tiles are spread evenly over the SMs: where there are fewer than fit at once, a block asks for so much shared memory that no SM takes more than its share.  (Left alone some take four and some
+// none: 2331 x 2304 bf16, 342 tiles, 6.9 us with room for four blocks to an SM and 5.8 with room for three; 4096 x 1024, 256 tiles, 5.5 and, with room for two, 4.6.)
+typedef void (*TileFn)(QuantArgs);
+static cudaError_t launch_tiles(TileFn fn, std::atomic<bool> (&ready)[64], const QuantArgs& a, cudaStream_t s) {
+  int dev = 0; cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+  constexpr int ROOM[3] = {200 << 10, 90 << 10, 55 << 10};      // beside 17 KiB of its own: one, two, three blocks in an SM's 228 KiB
+  if (!ready[dev]) {
+    const cudaError_t e = cudaFuncSetAttribute((const void*)fn, cudaFuncAttributeMaxDynamicSharedMemorySize, ROOM[0]);
+    if (e != cudaSuccess) return e;
+    ready[dev] = true;
+  }
+  const long long tiles = a.kc / 128 * (a.kr / 128), share = (tiles + 147) / 148;
+  return launch_pdl(fn, dim3((unsigned)tiles), 256, share <= 3 ? ROOM[share - 1] : 0, s, a);
+}
+template <typename T, bool VEC, bool ROWS, bool COLS, bool SQUARE> static cudaError_t tiles(const QuantArgs& a, cudaStream_t s) {
+  static std::atomic<bool> ready[64];
+  return launch_tiles(quant_tile_kernel<T, VEC, ROWS, COLS, SQUARE>, ready, a, s);
+}
 template <typename T, bool VEC>
 static cudaError_t quantize(const QuantArgs& a, int square, cudaStream_t s) {
   if (!a.t && !square) {
     const long long warps = (a.R + 127) / 128 * 128 * a.c4;
     return launch_pdl(quant_rows_kernel<T, VEC>, dim3((unsigned)((warps + 7) / 8)), 256, 0, s, a);
   }
-  const dim3 grid((unsigned)(a.kc / 128 * (a.kr / 128)));
-  if (square) return launch_pdl(a.t ? (a.q ? quant_tile_kernel<T, VEC, true, true, true> : quant_tile_kernel<T, VEC, false, true, true>) : quant_tile_kernel<T, VEC, true, false, true>, grid, 256, 0, s, a);
-  return launch_pdl(a.q ? quant_tile_kernel<T, VEC, true, true, false> : quant_tile_kernel<T, VEC, false, true, false>, grid, 256, 0, s, a);
+  if (square) return !a.t ? tiles<T, VEC, true, false, true>(a, s) : a.q ? tiles<T, VEC, true, true, true>(a, s) : tiles<T, VEC, false, true, true>(a, s);
+  return a.q ? tiles<T, VEC, true, true, false>(a, s) : tiles<T, VEC, false, true, false>(a, s);
 }
 
 }  // namespace piccl_ops
