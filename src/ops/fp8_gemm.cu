@@ -63,10 +63,9 @@ template <> struct OutPiece<float> {
     for (int j = 0; j < 8; j++) *reinterpret_cast<float4*>(row + ((j ^ (r & 7)) << 4)) = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
   }
 };
-// Rows of a result that do not start on 16 bytes, which no TMA store takes: a warp writes a row at a time, a word of 4 bytes a lane, from words of 16 rows that it has loaded (row by row, each
-// waiting for its load, a row took 200 clocks).  Rows of bf16 that begin in the middle of a word are moved by half a word, their first and last value written on their own.
-// 2331 x 50257 x 768: 150 us, where 50256 columns take 105.  What that costs are the sectors of which a piece writes a part: rows moved to 16-byte pieces in shared memory took 157, the ends of the pieces
-// alone 155, all but the ends 141.  left: columns that are there.
+// Rows of a result that do not start on 16 bytes, which no TMA store takes: a warp writes a row at a time, a word of 4 bytes a lane, from words of several rows that it has loaded.  Rows of bf16 that begin in the
+// middle of a word are moved by half a word, their first and last value written on their own.  What it costs is the instructions and their latencies, not the sectors that are written in part: 2331 x 50257 x 768
+// takes 127 us, 85 without this and 102 where 50256 columns go by TMA; with the questions which rows, columns and halves are there asked of each row 150, row by row 208.
 __device__ __forceinline__ uint32_t staged_word(const uint8_t* staging, int r, int lane) {
   return *reinterpret_cast<const uint32_t*>(staging + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4);
 }
@@ -80,8 +79,41 @@ __device__ __forceinline__ void store_rows(const uint8_t* staging, float* out, s
     for (int r = 0; r < 16; r++) if (r0 + r < rows && lane < left) out[(r0 + r) * stride + lane] = __uint_as_float(w[r]);
   }
 }
-__device__ __forceinline__ void store_rows(const uint8_t* staging, bf16* out, size_t stride, int rows, int left, int lane) {
+// A piece of which all rows and columns are there.  FIRST: its first row begins in the middle of a word, TURNS: every other row does.
+__device__ __forceinline__ void store_if(void* p, uint32_t x, bool there) { asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %2, 0;\n\t@p st.global.b32 [%0], %1;\n\t}" ::"l"(p), "r"(x), "r"((uint32_t)there) : "memory"); }
+__device__ __forceinline__ void store_half_if(void* p, uint32_t x, bool there) {
+  asm volatile("{\n\t.reg .pred p;\n\t.reg .b16 h;\n\tcvt.u16.u32 h, %1;\n\tsetp.ne.u32 p, %2, 0;\n\t@p st.global.b16 [%0], h;\n\t}" ::"l"(p), "r"(x), "r"((uint32_t)there) : "memory");
+}
+template <bool FIRST, bool TURNS> __device__ __forceinline__ void store_whole_rows(const uint8_t* staging, bf16* out, size_t stride, int lane) {
+  const bool inner = lane < 31, end = lane == 0 || lane == 31;
+  char* o = reinterpret_cast<char*>(out) + 4 * lane;
+  const int to_end = lane == 0 ? 0 : 2;
+#pragma unroll 1
+  for (int r0 = 0; r0 < 32; r0 += 8) {
+    uint32_t w[8], n[8];
 #pragma unroll
+    for (int r = 0; r < 8; r++) w[r] = staged_word(staging, r0 + r, lane);
+#pragma unroll
+    for (int r = 0; r < 8; r++) if (FIRST != (TURNS && (r & 1))) n[r] = __shfl_down_sync(0xffffffffu, w[r], 1);
+#pragma unroll
+    for (int r = 0; r < 8; r++, o += 2 * stride) {
+      if (FIRST != (TURNS && (r & 1))) {
+        store_if(o + 2, __funnelshift_r(w[r], n[r], 16), inner);
+        store_half_if(o + to_end, lane == 0 ? w[r] : w[r] >> 16, end);
+      } else *reinterpret_cast<uint32_t*>(o) = w[r];
+    }
+  }
+}
+__device__ __forceinline__ bool store_whole(const uint8_t* staging, bf16* out, size_t stride, int rows, int left, int lane) {
+  if (rows < 32 || left < 64) return false;
+  const bool first = reinterpret_cast<uintptr_t>(out) >> 1 & 1;
+  if (stride & 1) { if (first) store_whole_rows<true, true>(staging, out, stride, lane); else store_whole_rows<false, true>(staging, out, stride, lane); }
+  else if (first) store_whole_rows<true, false>(staging, out, stride, lane); else store_whole_rows<false, false>(staging, out, stride, lane);
+  return true;
+}
+__device__ __forceinline__ void store_rows(const uint8_t* staging, bf16* out, size_t stride, int rows, int left, int lane) {
+  if (store_whole(staging, out, stride, rows, left, lane)) return;
+#pragma unroll 1
   for (int r0 = 0; r0 < 32; r0 += 16) {
     uint32_t w[16], n[16];
 #pragma unroll
