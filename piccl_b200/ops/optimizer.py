@@ -16,6 +16,7 @@ One step at a time: steps of one optimiser on several streams need the order tha
 from __future__ import annotations
 
 import ctypes as C
+from bisect import bisect
 from typing import Optional, Sequence, Union
 
 import torch
@@ -54,6 +55,7 @@ class AdamW:
         written = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in (*params, *(w for w in masters if w is not None)) if t.numel())
         if any(a[1] > b[0] for a, b in zip(written, written[1:])):
             raise ValueError("AdamW: parameters or masters that overlap")
+        self._written = written
         self.params, self.masters, self.decay, self.bits, self.seed = params, masters, [bool(d) for d in decay], bits, int(seed) & 0xFFFFFFFF
         self.places, block = [], 0                    # (first element in m and v, elements) of each tensor
         for p in params:
@@ -87,6 +89,9 @@ class AdamW:
                 raise ValueError(f"AdamW: a contiguous gradient of {n} elements, bf16 or fp32, on {self.device} wanted, got {g.dtype} {tuple(g.shape)} on {g.device}")
             if n == 0:
                 continue
+            at = bisect(self._written, (g.data_ptr() + n * g.element_size() - 1, 1 << 64)) - 1      # the last of them that begins before the gradient's end
+            if at >= 0 and self._written[at][1] > g.data_ptr():
+                raise ValueError("AdamW: a gradient that overlaps a parameter or a master")
             flags = _DECAY * d | _P_F32 * (w is None) | _G_F32 * (g.dtype == torch.float32)
             if all(t is None or t.data_ptr() % (8 * t.element_size()) == 0 for t in (p, w, g)):
                 flags |= _WORDS

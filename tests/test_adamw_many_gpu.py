@@ -243,6 +243,19 @@ def test_gpt2_with_moments_in_8_bits():
         GPT2(cfg, adam_bits=16)
 
 
+def test_gradients_beside_their_parameters_in_a_buffer():
+    """Next to each other is fine, overlapping is refused: other lanes would read what one has written."""
+    from piccl_b200.ops.optimizer import AdamW
+    buf = torch.ones(64, device="cuda")
+    opt = AdamW([buf[16:32], buf[40:48]], [buf[0:16], buf[32:40]])
+    opt.set_grads([buf[48:64], buf[8:16]])
+    for grads in ([buf[16:32], buf[32:40]], [buf[8:24], buf[32:40]], [buf[24:40], buf[32:40]], [buf[0:16], buf[47:55]], [buf[0:16], buf[33:41]], [torch.zeros(16, device="cuda"), buf.view(torch.bfloat16)[94:102]]):
+        with pytest.raises(ValueError, match="overlap"):
+            opt.set_grads(grads)
+    opt.step(0.0, wd=0.0)
+    assert bool((buf == 1).all()) and torch.equal(opt.moments(0)[0], torch.full((16,), torch.tensor(1 - 0.9, dtype=torch.float32).item(), device="cuda"))
+
+
 def test_refusals_on_the_gpu():
     from piccl_b200.ops.optimizer import AdamW
     p, g = torch.ones(16, device="cuda"), torch.ones(16, device="cuda")
