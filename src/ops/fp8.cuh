@@ -10,7 +10,7 @@
 
 namespace piccl_ops {
 
-// fp8_few.cu: products of at most 64 rows
+// fp8_few.cu: products of at most 32 rows
 bool fp8_few_takes(int M, int N, long long K, bool rounded);
 int fp8_few(const bf16* x, long long stride, const void* a, const void* sa, const void* b, const void* sb, const void* bias, void* out, int f32, int M, int N, int K, void* stream);
 

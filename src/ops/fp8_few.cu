@@ -1,4 +1,4 @@
-// The products of fp8_gemm.cu for at most 64 rows, as in decoding: C[M, N] = A[M, K] B[N, K]^T + bias, bound by the bytes of B.
+// The products of fp8_gemm.cu for at most 32 rows, as in decoding: C[M, N] = A[M, K] B[N, K]^T + bias, bound by the bytes of B.
 //
 // A block has 16 or 32 rows of B, its eight warps take the k-blocks of 128 in turn: a warp reads its part of B straight into the fragments of mma.sync (B's rows are the fragment's 16 rows, A's
 // rows its 8 columns; k may stand in any order that both sides share, so a lane's 16 bytes are contiguous), sums a block of 128 and adds it to its sums in fp32, scaled by the two powers of two.  The
