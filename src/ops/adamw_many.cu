@@ -6,7 +6,7 @@
 // 2^-18 of a block's largest value, 2^-36 of the largest v) and is what the update divides by.  Both are rounded stochastically, up with the probability of the part cut off.
 // Rounded to nearest they would stand still: with b2 = 0.999 a root changes by 0.05 % a step, and e4m3's half step is 3 to 6 %.  A root that is not zero does not become zero, or the
 // update of an element whose gradients are 2^-18 of its block's largest would divide by eps alone.  The random bits are a hash of the element's place, the step and a seed, so a run can be
-// repeated bit by bit; for the same reason the state's arithmetic is in single roundings (no fma).
+// repeated bit by bit; for the same reason the state's arithmetic is in single roundings (no fma: sum2_alone).
 #include "fp8.cuh"
 
 namespace piccl_ops {
@@ -23,9 +23,13 @@ struct AdamArgs {
   const AdamTensor* tensors; const int* owner; long long blocks;      // owner: the tensor of each block
   void *m, *v; uint8_t *ms, *vs;
   float lr, b1, c1, b2, c2, eps, wd, lb1, lb2;      // c: 1 - b; lb: logarithms
-  float gscale; const float* gscale_dev;
+  float gscale, one; const float* gscale_dev;      // one: 1
   int* step; unsigned* ticket; uint32_t seed;
 };
+
+// a + b where a is a product that has been rounded.  The compiler makes one fma of a packed product and a packed sum, whatever their rounding modes say (mul.rn.f32x2, add.rn.f32x2); of a product and
+// an fma by a factor that it does not know it cannot.
+__device__ __forceinline__ f32x2 sum2_alone(f32x2 a, f32x2 b, float one) { return fma2(a, both2(one), b); }
 
 __device__ __forceinline__ uint32_t random_bits(uint32_t place, uint32_t key) {
   uint32_t h = place * 0x9E3779B9u + key;      // the golden ratio, then the roots of 3 and 2: odd numbers without a pattern
@@ -160,8 +164,8 @@ struct AdamStep {
     for (int k = 0; k < E / 2; k++) {
       f32x2 g = flags & ADAM_G_F32 ? pack2(__uint_as_float(gw[2 * k]), __uint_as_float(gw[2 * k + 1])) : pack2(__uint_as_float(gw[k] << 16), __uint_as_float(gw[k] & 0xffff0000u));
       g = mul2(g, both2(gscale));
-      m[k] = add2(mul2(both2(a.b1), m[k]), mul2(both2(a.c1), g));
-      v[k] = add2(mul2(both2(a.b2), v[k]), mul2(mul2(both2(a.c2), g), g));
+      m[k] = sum2_alone(mul2(both2(a.b1), m[k]), mul2(both2(a.c1), g), a.one);
+      v[k] = sum2_alone(mul2(both2(a.b2), v[k]), mul2(mul2(both2(a.c2), g), g), a.one);
       float x, y, d, e; unpack2(v[k], x, y);
       x = adam_root<BITS8>(x); y = adam_root<BITS8>(y);
       root[k] = pack2(x, y);
@@ -307,7 +311,7 @@ int piccl_ops_adamw_many(const void* tensors, const int* owner, long long blocks
   if ((blocks && (!tensors || !owner || !m || !v || (bits8 && (!ms || !vs)))) || !step || !ticket) return -2;
   if ((reinterpret_cast<uintptr_t>(m) | reinterpret_cast<uintptr_t>(v)) & 31) return -2;      // the kernel's accesses of 32 bytes
   AdamArgs a{static_cast<const AdamTensor*>(tensors), owner, blocks, m, v, (uint8_t*)ms, (uint8_t*)vs, lr, (float)b1, (float)(1 - b1), (float)b2, (float)(1 - b2), eps, wd, (float)log(b1), (float)log(b2),
-             gscale, gscale_dev, step, ticket, seed};
+             gscale, 1.f, gscale_dev, step, ticket, seed};
   const long long want = (blocks + 15) / 16, most = 148 * 3;
   const dim3 grid((unsigned)(want < 1 ? 1 : want < most ? want : most));
   const cudaError_t e = launch_pdl(bits8 ? adamw_many8_kernel : adamw_many_kernel, grid, 256, 0, (cudaStream_t)stream, a);
