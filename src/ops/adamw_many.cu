@@ -62,23 +62,27 @@ template <bool ROOT> __device__ __forceinline__ float stochastic_any(float x, fl
 // The byte of a block whose largest value is the root of v: the smallest s for which v <= (448 * 2^s)^2 = 1.53125 * 2^(17 + 2 s).  (A root rounded to fp32 is above 448 * 2^s exactly
 // where v is above that, so this is the byte of correctly rounded roots.)
 __device__ __forceinline__ uint32_t scale_byte_of_root(uint32_t v_bits) {
-  const int e = (int)((v_bits + (0x7fffffu - 0x440000u)) >> 23) - 127 - 17, s = 127 + ((e + 1) >> 1);
-  return v_bits < 0x00800000u ? 1u : (uint32_t)s;
+  if (v_bits < 0x00800000u) return scale_byte(__float_as_uint(__fsqrt_rn(__uint_as_float(v_bits))));      // the exponent of a v below 2^-126 is not in its bits
+  const int e = (int)((v_bits + (0x7fffffu - 0x440000u)) >> 23) - 127 - 17;
+  return (uint32_t)(127 + ((e + 1) >> 1));
 }
 __device__ __forceinline__ uint2 e4m3_bytes(const float (&t)[8]) {
   return make_uint2(e4m3_four(t[0], t[1], t[2], t[3]), e4m3_four(t[4], t[5], t[6], t[7]));
 }
 // Eight moments and roots of a block, by 16 lanes -> their bytes and the block's two.  All lanes of a warp call it together (votes and shuffles among a part of them cost a barrier each), and both
 // maxima are found side by side: one after the other, each behind its own votes, the latencies of shuffles were a third of the kernel's time.
-__device__ __forceinline__ void round_moments(const f32x2 (&m2)[4], const f32x2 (&v2)[4], const f32x2 (&r2)[4], const uint32_t (&random)[8], uint2& m_out, uint2& v_out, uint32_t& m_byte, uint32_t& v_byte) {
-  float m[8], v[8], r[8];
+// What is held is the correctly rounded root's: whether the random bits carry can hang on its last bit, and a carry is a whole step of e4m3.  r2 are approximate roots, off by less than four units in the last place (2^-23 is
+// two, and half a one is the rounding), so they decide where the sum is at least that far from a carry.  Nearer ones, eight in 2^20, and whatever is below 2^-6, are rounded again from roots by
+// __fsqrt_rn: GPT-2 medium 1166 us (1111 with approximate roots alone, 1220 with __fsqrt_rn throughout; 1178 with the random bits kept for the second rounding).
+__device__ __forceinline__ void round_moments(const f32x2 (&m2)[4], const f32x2 (&v2)[4], const f32x2 (&r2)[4], float r_least, uint32_t place, uint32_t key, uint2& m_out, uint2& v_out, uint32_t& m_byte, uint32_t& v_byte) {
+  float m[8], v[8];
 #pragma unroll
-  for (int i = 0; i < 4; i++) { unpack2(m2[i], m[2 * i], m[2 * i + 1]); unpack2(v2[i], v[2 * i], v[2 * i + 1]); unpack2(r2[i], r[2 * i], r[2 * i + 1]); }
-  float m_most = fabsf(m[0]), m_least = fabsf(m[0]), v_most = v[0], r_least = r[0];
+  for (int i = 0; i < 4; i++) { unpack2(m2[i], m[2 * i], m[2 * i + 1]); unpack2(v2[i], v[2 * i], v[2 * i + 1]); }
+  float m_most = fabsf(m[0]), m_least = fabsf(m[0]), v_most = v[0];
 #pragma unroll
   for (int e = 1; e < 8; e += 2) {
     m_most = max3_nan(m_most, fabsf(m[e]), fabsf(m[(e + 1) % 8])); m_least = min3(m_least, fabsf(m[e]), fabsf(m[(e + 1) % 8]));
-    v_most = max3_nan(v_most, v[e], v[(e + 1) % 8]); r_least = min3(r_least, r[e], r[(e + 1) % 8]);
+    v_most = max3_nan(v_most, v[e], v[(e + 1) % 8]);
   }
   uint32_t m_top = __float_as_uint(m_most), v_top = __float_as_uint(v_most);
   bool odd = __any_sync(0xffffffffu, max(m_top, v_top) >= kInf);
@@ -94,16 +98,35 @@ __device__ __forceinline__ void round_moments(const f32x2 (&m2)[4], const f32x2 
   }
   m_byte = scale_byte(m_top); v_byte = scale_byte_of_root(v_top);
   const float fm = scale_inverse(m_byte), fr = scale_inverse(v_byte);
+  uint32_t random[8];
+#pragma unroll
+  for (int e = 0; e < 8; e++) random[e] = random_bits(place + e, key);
   odd = __any_sync(0xffffffffu, odd || fminf(m_least * fm, r_least * fr) < 0.015625f);
   float a[8], b[8];
 #pragma unroll
   for (int i = 0; i < 4; i++) { unpack2(mul2(m2[i], both2(fm)), a[2 * i], a[2 * i + 1]); unpack2(mul2(r2[i], both2(fr)), b[2 * i], b[2 * i + 1]); }
   if (odd) {
 #pragma unroll
-    for (int e = 0; e < 8; e++) { a[e] = stochastic_any<false>(m[e], a[e], random[e]); b[e] = stochastic_any<true>(r[e], b[e], random[e]); }
+    for (int e = 0; e < 8; e++) a[e] = stochastic_any<false>(m[e], a[e], random[e]);
   } else {
+    uint32_t near = 0xffffffffu;                            // the low 20 bits of the sums, as distances from four below a carry
 #pragma unroll
-    for (int e = 0; e < 8; e++) { a[e] = stochastic<false>(a[e], random[e]); b[e] = stochastic<true>(b[e], random[e]); }
+    for (int e = 0; e < 8; e += 2) {
+      uint32_t sum[2];
+#pragma unroll
+      for (int i = 0; i < 2; i++) {
+        a[e + i] = stochastic<false>(a[e + i], random[e + i]);
+        sum[i] = __float_as_uint(b[e + i]) + random_part<true>(random[e + i]) + 4u;
+        b[e + i] = __uint_as_float(sum[i] & 0xfff00000u);
+      }
+      near = __vimin3_u32(near, sum[0] << 12, sum[1] << 12);
+    }
+    odd = __any_sync(0xffffffffu, near < 8u << 12);
+  }
+  if (odd) {
+    asm volatile("" : "+r"(place));                         // the bits are computed again, not kept
+#pragma unroll
+    for (int e = 0; e < 8; e++) { const float root = __fsqrt_rn(v[e]); b[e] = stochastic_any<true>(root, root * fr, random_bits(place + e, key)); }
   }
   m_out = e4m3_bytes(a); v_out = e4m3_bytes(b);
 }
@@ -134,7 +157,7 @@ __device__ __forceinline__ void adam_find(const AdamArgs& a, long long block, Ad
   c.p = q.flags & ADAM_P_F32 ? nullptr : static_cast<bf16*>(q.p); c.master = q.flags & ADAM_P_F32 ? static_cast<float*>(q.p) : q.master;
   c.end = q.block + (q.n + 127) / 128;
 }
-// The root of v: in 8 bits the approximate one (2^-23; what it is rounded to has 2^-4), in which v below 2^-126 counts as zero
+// The root of v that the update divides by: in 8 bits the approximate one (to 2^-23, less than the division's own two units; zero for v below 2^-126, which the caller looks after)
 template <bool BITS8> __device__ __forceinline__ float adam_root(float v) {
   float r;
   if (BITS8) asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v)); else r = __fsqrt_rn(v);
@@ -157,8 +180,8 @@ struct AdamStep {
     __syncthreads();                                       // every thread has read *step
     if (threadIdx.x == 0 && atomicAdd(a.ticket, 1u) == gridDim.x - 1) { *a.ticket = 0; atomicAdd(a.step, 1); }
   }
-  // moments, roots and weights of E elements; w: as bits
-  template <bool BITS8, int E> __device__ __forceinline__ void update(const AdamArgs& a, int flags, const uint32_t (&gw)[E], uint32_t (&w)[E], f32x2 (&m)[E / 2], f32x2 (&v)[E / 2], f32x2 (&root)[E / 2]) const {
+  // moments, roots and weights of E elements; w: as bits; least: in 8 bits, of the roots
+  template <bool BITS8, int E> __device__ __forceinline__ void update(const AdamArgs& a, int flags, const uint32_t (&gw)[E], uint32_t (&w)[E], f32x2 (&m)[E / 2], f32x2 (&v)[E / 2], f32x2 (&root)[E / 2], float& least) const {
     const float keep = 1.f - a.lr * (flags & ADAM_DECAY ? a.wd : 0.f);
 #pragma unroll
     for (int k = 0; k < E / 2; k++) {
@@ -166,9 +189,21 @@ struct AdamStep {
       g = mul2(g, both2(gscale));
       m[k] = sum2_alone(mul2(both2(a.b1), m[k]), mul2(both2(a.c1), g), a.one);
       v[k] = sum2_alone(mul2(both2(a.b2), v[k]), mul2(mul2(both2(a.c2), g), g), a.one);
-      float x, y, d, e; unpack2(v[k], x, y);
+      float x, y; unpack2(v[k], x, y);
       x = adam_root<BITS8>(x); y = adam_root<BITS8>(y);
+      if (BITS8) least = k ? min3(least, x, y) : fminf(x, y);
       root[k] = pack2(x, y);
+    }
+    if (BITS8 && least == 0.f) {                            // zero, or below 2^-126, where the approximate root is zero
+#pragma unroll
+      for (int k = 0; k < E / 2; k++) {
+        float x, y, p, q; unpack2(v[k], x, y); unpack2(root[k], p, q);
+        root[k] = pack2(p == 0.f ? __fsqrt_rn(x) : p, q == 0.f ? __fsqrt_rn(y) : q);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < E / 2; k++) {
+      float x, y, d, e;
       unpack2(fma2(root[k], both2(rc2), both2(a.eps)), d, e);
       unpack2(mul2(m[k], both2(lr1)), x, y);
       w[2 * k] = __float_as_uint(fmaf(__uint_as_float(w[2 * k]), keep, -div_approx(x, d)));
@@ -227,7 +262,8 @@ __global__ void __launch_bounds__(256, 3) adamw_many_kernel(const AdamArgs a) {
       load_words(now.master + i, w);
       if (now.flags & ADAM_G_F32) load_words(gradients(now, i), gw); else load_words(gradients(now, i), reinterpret_cast<uint32_t (&)[E / 2]>(gw));
     } else load_some(gradients(now, i), now.master + i, left, now.flags, gw, w);
-    step.update<false>(a, now.flags, gw, w, m, v, root);
+    float unused;
+    step.update<false>(a, now.flags, gw, w, m, v, root, unused);
     store_weights(now.master + i, now.p ? now.p + i : nullptr, left, words, w);
     store_words(static_cast<float*>(a.m) + s, reinterpret_cast<const uint32_t (&)[E]>(m));
     store_words(static_cast<float*>(a.v) + s, reinterpret_cast<const uint32_t (&)[E]>(v));
@@ -236,7 +272,7 @@ __global__ void __launch_bounds__(256, 3) adamw_many_kernel(const AdamArgs a) {
 }
 
 // Moments in 8 bits: a lane has eight elements, sixteen lanes a block, a warp two blocks.  16 bytes an element (868 us of memory for GPT-2 medium) and about as much arithmetic: two roundings, a root and a division each.
-// 1115 us there, 5.1 TB/s; without the prefetch of the next block's lines 1245, with 16 warps to an SM in place of 24 1395.
+// 1166 us there, 4.9 TB/s; before the held roots were rounded correctly 1111, without the prefetch of the next block's lines 1245, with 16 warps to an SM in place of 24 1395.
 __global__ void __launch_bounds__(256, 3) adamw_many8_kernel(const AdamArgs a) {
   constexpr int E = 8;
   pdl_begin();
@@ -274,11 +310,9 @@ __global__ void __launch_bounds__(256, 3) adamw_many8_kernel(const AdamArgs a) {
     }
 #pragma unroll
     for (int k = 0; k < 4; k++) v[k] = mul2(v[k], v[k]);
-    step.update<true>(a, now.flags, gw, w, m, v, root);
+    float least;                                            // of the roots
+    step.update<true>(a, now.flags, gw, w, m, v, root, least);
     store_weights(now.master + i, now.p ? now.p + i : nullptr, left, words, w);
-    uint32_t random[E];
-#pragma unroll
-    for (int e = 0; e < E; e++) random[e] = random_bits((uint32_t)s + e, step.key);
     if (left < E) {                                         // what lies beyond the tensor stays zero
 #pragma unroll
       for (int k = 0; k < 4; k++)
@@ -288,7 +322,7 @@ __global__ void __launch_bounds__(256, 3) adamw_many8_kernel(const AdamArgs a) {
         }
     }
     uint2 om, ov;
-    round_moments(m, v, root, random, om, ov, mb, vb);
+    round_moments(m, v, root, least, (uint32_t)s, step.key, om, ov, mb, vb);
     if (!there) continue;
     *reinterpret_cast<uint2*>(static_cast<uint8_t*>(a.m) + s) = om;
     *reinterpret_cast<uint2*>(static_cast<uint8_t*>(a.v) + s) = ov;

@@ -1,8 +1,134 @@
 """The moments of AdamW, step after step against their definition in plain single-precision operations, which never takes over what the kernel holds."""
+import math
+
 import pytest
 import torch
 
 pytestmark = pytest.mark.gpu
+
+HALF = 2.0 ** -24          # half a step of fp32, relative to the value
+
+
+def _random(n, seed, step):
+    """The definition's 32 random bits for each place"""
+    mask = 0xFFFFFFFF
+    h = torch.arange(n, device="cuda").mul_(0x9E3779B9).add_(seed + step * 0x9E3779B9).bitwise_and_(mask)
+    h = ((h ^ (h >> 16)) * 0xBB67AE85) & mask
+    h = ((h ^ (h >> 15)) * 0x6A09E667) & mask
+    return h ^ (h >> 16)
+
+
+def _hold(x, u, positive):
+    """fp32 values of whole blocks of 128 -> what the bytes stand for (before the scale) and the scales' bytes: rounded up with the probability of the part cut off"""
+    b = x.view(-1, 128)
+    top = torch.where(b.isfinite(), b.abs(), 0.0).amax(1)
+    byte = (((top.view(torch.int32) + 0x1FFFFF) >> 23) - 8).clamp(min=1)
+    t = b * ((254 - byte) << 23).view(torch.float32)[:, None]
+    a = t.abs()
+    low = torch.where(a < 2.0 ** -6, 2.0 ** -6, 0.0)          # below, e4m3's steps are those of [2^-6, 2^-5)
+    z = (a + low).view(torch.int32) + (u.view(-1, 128) << 4).to(torch.int32)
+    z = (z & ~0xFFFFF).view(torch.float32) - low
+    if positive:
+        z = torch.where(a > 0, z.clamp(min=2.0 ** -9), z)
+    return z.copysign(t).view(-1), byte
+
+
+def _value(z, byte):
+    return (z.view(-1, 128) * (byte << 23).view(torch.float32)[:, None]).view(-1)
+
+
+class _Plain:
+    """The state as fp32 tensors of whole blocks; the weights follow it in fp64, with a bound on what fp32 may lose from them"""
+
+    def __init__(self, w):
+        n = w.numel()
+        full = (n + 127) // 128 * 128
+        self.n, self.w, self.allowed = n, w.double(), torch.zeros(n, dtype=torch.float64, device="cuda")
+        self.zm, self.zr = torch.zeros(full, device="cuda"), torch.zeros(full, device="cuda")
+        self.em, self.er = (torch.ones(full // 128, dtype=torch.int32, device="cuda") for _ in range(2))
+        self.t = 0
+
+    def step(self, g, seed, lr, b1, b2, eps, wd, gscale):
+        self.t += 1
+        x = torch.zeros_like(self.zm)
+        x[:self.n] = g.float() * gscale
+        m, r = _value(self.zm, self.em), _value(self.zr, self.er)
+        m = m * b1 + x * (1.0 - b1)
+        v = (r * r) * b2 + (x * (1.0 - b2)) * x
+        u = _random(x.numel(), seed, self.t)
+        self.zm, self.em = _hold(m, u & 0xFFFF, False)
+        self.zr, self.er = _hold(v.sqrt(), u >> 16, True)
+        m, v = m[:self.n].double(), v[:self.n].double()
+        change = lr * (m / (1 - b1 ** self.t)) / ((v / (1 - b2 ** self.t)).sqrt() + eps)
+        after = self.w * (1 - lr * wd) - change
+        # 13 half steps of the change: three of each of 1 - b^t and its reciprocal, one of lr, two of an approximate root, one of eps, four of a quotient that is right to two steps (and 20 stand here); one of
+        # the factor of the weight, one of the result
+        self.allowed += 2 * HALF * (self.w.abs() + after.abs() + 10 * change.abs())
+        self.w = after
+
+
+def _compare(opt, plain, p):
+    assert torch.equal(opt.m_scales.int(), plain.em) and torch.equal(opt.v_scales.int(), plain.er)
+    assert torch.equal(opt.m.float(), plain.zm), int((opt.m.float() != plain.zm).sum())
+    assert torch.equal(opt.v.float(), plain.zr), int((opt.v.float() != plain.zr).sum())
+    off = (p.double() - plain.w).abs()
+    assert bool((off <= plain.allowed).all()), float((off / plain.allowed.clamp(min=1e-300)).max())
+
+
+def test_eight_steps_side_by_side():
+    """The state is the definition's bit for bit, with the correctly rounded root (one unit in the last place moves a held root by a whole step of e4m3 where it tips the carry, in an element
+    of 10^6 a step, and the next step divides by that), and so the weights stay where sums in fp32 put them."""
+    from piccl_b200.ops.optimizer import AdamW
+    n, seed = (1 << 25) + 77, 21
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    size = torch.exp(torch.randn(n // 128 + 1, 1, generator=gen, device="cuda") - 9.0).expand(-1, 128).reshape(-1)[:n]
+    w = torch.randn(n, generator=gen, device="cuda") * 0.02
+    p, g = w.clone(), torch.empty(n, dtype=torch.bfloat16, device="cuda")
+    opt, plain = AdamW([p], [g], bits=8, seed=seed), _Plain(w)
+    del w
+    for _ in range(8):
+        g.copy_(torch.randn(n, generator=gen, device="cuda") * size)
+        g[1 << 20:(1 << 20) + 500] = 0
+        opt.step(3e-4, 0.9, 0.95, 1e-8, 0.1, gscale=0.7)
+        plain.step(g, seed, 3e-4, 0.9, 0.95, 1e-8, 0.1, 0.7)
+        _compare(opt, plain, p)
+
+
+@pytest.mark.parametrize("eps", [0.0, 1e-8])
+@pytest.mark.parametrize("size", [2.0 ** -62, 2.0 ** -66, 2.0 ** -70])
+def test_second_moments_below_the_normal_numbers(size, eps):
+    """v is below 2^-126, its root a normal number: no root that is not zero becomes zero, and the update divides by it."""
+    from piccl_b200.ops.optimizer import AdamW
+    n, seed = 128 * 300 + 5, 3
+    gen = torch.Generator(device="cuda").manual_seed(9)
+    w = torch.randn(n, generator=gen, device="cuda")
+    p, g = w.clone(), torch.zeros(n, device="cuda")
+    opt, plain = AdamW([p], [g], bits=8, seed=seed), _Plain(w)
+    for _ in range(3):
+        g.copy_((torch.rand(n, generator=gen, device="cuda") + 0.5) * torch.randn(n, generator=gen, device="cuda").sign() * size)
+        if eps:
+            g[128:256] = 0          # nothing there
+            g[260:300] *= 2.0 ** 40          # beside values far above
+        opt.step(1e-3, 0.9, 0.95, eps, 0.1)
+        plain.step(g, seed, 1e-3, 0.9, 0.95, eps, 0.1, 1.0)
+        assert bool((opt.v.float()[:n][g != 0] > 0).all())
+        _compare(opt, plain, p)
+
+
+def test_the_largest_gradients():
+    """Second moments up to fp32's largest."""
+    from piccl_b200.ops.optimizer import AdamW
+    n, seed = 128 * 40 + 3, 4
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    w = torch.randn(n, generator=gen, device="cuda")
+    p, g = w.clone(), torch.zeros(n, device="cuda")
+    opt, plain = AdamW([p], [g], bits=8, seed=seed), _Plain(w)
+    for _ in range(3):
+        g.copy_(torch.randn(n, generator=gen, device="cuda").clamp(-4, 4) * 4.0e18)
+        opt.step(1e-3, 0.9, 0.95, 1e-8, 0.1)
+        plain.step(g, seed, 1e-3, 0.9, 0.95, 1e-8, 0.1, 1.0)
+        _compare(opt, plain, p)
+    assert math.isfinite(float(p.abs().max()))
 
 
 def test_moments_in_32_bits_are_rounded_one_operation_at_a_time():
