@@ -11,6 +11,7 @@
 #include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/Device.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include "../ops/piccl_ops.h"
 
@@ -78,7 +79,7 @@ PyObject* answer(int rc, int launches, const char* what) {
   return nullptr;
 }
 template <class F> PyObject* guarded(F f) {
-  try { return f(); } catch (const std::exception& e) { PyErr_SetString(PyExc_RuntimeError, e.what()); return nullptr; }
+  try { return f(); } catch (...) { torch::translate_exception_to_python(std::current_exception()); return nullptr; }      // out of memory stays torch.OutOfMemoryError
 }
 PyObject* no() { return PyLong_FromLong(0); }
 
