@@ -10,6 +10,8 @@ step can be captured into a CUDA graph and replayed; `gscale` multiplies the gra
 Moments are the optimiser's own: `m` and `v`, flat, each tensor from a multiple of 128 elements on (`places`).  In 8 bits they are e4m3 values with
 a power of two for each block of 128 (`m_scales`, `v_scales`: byte e stands for 2^(e - 127)), v as its root, and are rounded stochastically, by bits that
 depend on the element's place, the step and `seed` alone: 2.02 bytes a parameter in place of 8.  Values that are not finite are held as NaN.
+These tensors, `step_dev` and `seed` are what captured steps go on reading and cannot be exchanged: a state is loaded into them (`load_state`, or `opt.m.copy_(...)`).  Parameters, masters and gradients stay where
+they are too; a step after one of them has been given other memory (`p.data = ...`) is refused.
 
 One step at a time: steps of one optimiser on several streams need the order that any two writers of the same tensors need.
 """
@@ -17,7 +19,7 @@ from __future__ import annotations
 
 import ctypes as C
 from bisect import bisect
-from typing import Optional, Sequence, Union
+from typing import Mapping, Optional, Sequence, Union
 
 import torch
 
@@ -43,7 +45,7 @@ class AdamW:
         decay = [True] * len(params) if decay is None else list(decay)
         if not params or not len(params) == len(grads) == len(masters) == len(decay):
             raise ValueError(f"AdamW: {len(params)} parameters, {len(grads)} gradients, {len(masters)} masters, {len(decay)} decays")
-        self.device = params[0].device
+        self._device = params[0].device
         for p, w in zip(params, masters):
             if p.dtype not in (torch.bfloat16, torch.float32) or (p.dtype == torch.float32) != (w is None):
                 raise ValueError("AdamW: parameters are bf16 with a master or fp32 without")
@@ -56,25 +58,47 @@ class AdamW:
         if any(a[1] > b[0] for a, b in zip(written, written[1:])):
             raise ValueError("AdamW: parameters or masters that overlap")
         self._written = written
-        self.params, self.masters, self.decay, self.bits, self.seed = params, masters, [bool(d) for d in decay], bits, int(seed) & 0xFFFFFFFF
-        self.places, block = [], 0                    # (first element in m and v, elements) of each tensor
+        self._params, self._masters, self._decay, self._bits, self._seed = tuple(params), tuple(masters), tuple(bool(d) for d in decay), bits, int(seed) & 0xFFFFFFFF
+        self._fixed = [(t, t.data_ptr()) for t in (*params, *masters) if t is not None]
+        places, block = [], 0                         # (first element in m and v, elements) of each tensor
         for p in params:
-            self.places.append((block * 128, p.numel()))
+            places.append((block * 128, p.numel()))
             block += (p.numel() + 127) // 128
-        self.blocks = block
+        self._places, self._blocks = tuple(places), block
         zeros = lambda n, dtype: torch.zeros(n, dtype=dtype, device=self.device)  # noqa: E731
         kind = E4M3 if bits == 8 else torch.float32
-        self.m, self.v = zeros(block * 128, kind), zeros(block * 128, kind)
-        self.m_scales, self.v_scales = (torch.ones(block, dtype=torch.uint8, device=self.device) for _ in range(2)) if bits == 8 else (None, None)
-        self.step_dev, self._ticket = zeros(1, torch.int32), zeros(1, torch.int32)
+        self._m, self._v = zeros(block * 128, kind), zeros(block * 128, kind)
+        self._m_scales, self._v_scales = (torch.ones(block, dtype=torch.uint8, device=self.device) for _ in range(2)) if bits == 8 else (None, None)
+        self._step_dev, self._ticket = zeros(1, torch.int32), zeros(1, torch.int32)
         lengths = [(n + 127) // 128 for _, n in self.places if n]
         self._owner = torch.repeat_interleave(torch.arange(len(lengths), dtype=torch.int32), torch.tensor(lengths, dtype=torch.int64)).to(self.device)      # the tensor of each block
         self._table = None
+        self._calls = _native_calls()
+        self._fast = self._calls.adamw_step if self._calls else None
         self.set_grads(grads)
-        fast = _native_calls()
-        self._fast = fast.adamw_step if fast else None
-        self._handle = fast.adamw(self.device.index, self._table.data_ptr(), self._owner.data_ptr(), block, bits == 8, self.m.data_ptr(), self.v.data_ptr(), _ptr(self.m_scales) or 0, _ptr(self.v_scales) or 0,
-                                  self.step_dev.data_ptr(), self._ticket.data_ptr(), self.seed) if fast else None
+
+    # what the table and the native handle were made from, and captured steps go on reading: not to be set
+    (device, params, masters, grads, decay, bits, seed, places, blocks, m, v, m_scales, v_scales, step_dev) = (
+        property(lambda self, name=name: getattr(self, name)) for name in ("_device", "_params", "_masters", "_grads", "_decay", "_bits", "_seed", "_places", "_blocks", "_m", "_v", "_m_scales", "_v_scales", "_step_dev"))
+
+    def state(self) -> dict[str, torch.Tensor]:
+        """The optimiser's own tensors, by name: what has to be kept, beside the parameters and masters, to go on with the next step."""
+        names = ("m", "v", "step_dev", *(("m_scales", "v_scales") if self.bits == 8 else ()))
+        return {name: getattr(self, name) for name in names}
+
+    def load_state(self, state: Mapping[str, torch.Tensor]) -> None:
+        """Takes over the values of another's `state`: of as many bits, over tensors of the same sizes (and made with the same `seed`, if its steps are to be repeated bit by bit)."""
+        mine = self.state()
+        for name, t in mine.items():
+            if name not in state or state[name].dtype != t.dtype or state[name].shape != t.shape:
+                raise ValueError(f"AdamW: {name} of {t.numel()} {t.dtype} wanted, got {'none' if name not in state else (state[name].dtype, tuple(state[name].shape))}")
+        for name, t in mine.items():
+            t.copy_(state[name])
+
+    @staticmethod
+    def _stay(tensors) -> None:
+        if any(t.data_ptr() != at for t, at in tensors):
+            raise ValueError("AdamW: a parameter, master or gradient is not where it was (it has been given other memory)")
 
     def set_grads(self, grads: Sequence[torch.Tensor]) -> None:
         """Other tensors to take the gradients from, from the next step on (a copy of addresses to the device; not within a capture)."""
@@ -83,6 +107,7 @@ class AdamW:
             raise ValueError(f"AdamW: {len(self.params)} gradients wanted, got {len(grads)}")
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("AdamW: gradients cannot be exchanged within a capture")
+        self._stay(self._fixed)
         records = []
         for p, w, g, d, (first, n) in zip(self.params, self.masters, grads, self.decay, self.places):
             if g.dtype not in (torch.bfloat16, torch.float32) or g.numel() != n or not g.is_contiguous() or g.device != self.device:
@@ -96,12 +121,16 @@ class AdamW:
             if all(t is None or t.data_ptr() % (8 * t.element_size()) == 0 for t in (p, w, g)):
                 flags |= _WORDS
             records.append(_Tensor(p.data_ptr(), 0 if w is None else w.data_ptr(), g.data_ptr(), n, first // 128, flags, 0))
-        self.grads = grads
+        self._grads = tuple(grads)
         raw = torch.frombuffer(bytearray((_Tensor * max(1, len(records)))(*records)), dtype=torch.uint8)
         if self._table is None:
             self._table = raw.to(self.device)
         else:
             self._table.copy_(raw)                    # in place: captured steps read it, and steps before on this stream have
+        self._stand = self._fixed + [(g, g.data_ptr()) for g in grads]
+        if self._calls:
+            self._handle = self._calls.adamw(self.device.index, self._table.data_ptr(), self._owner.data_ptr(), self.blocks, self.bits == 8, self.m.data_ptr(), self.v.data_ptr(), _ptr(self.m_scales) or 0,
+                                             _ptr(self.v_scales) or 0, self.step_dev.data_ptr(), self._ticket.data_ptr(), self.seed, tuple(t for t, _ in self._stand))
 
     def step(self, lr: float, b1: float = 0.9, b2: float = 0.95, eps: float = 1e-8, wd: float = 0.1, gscale: Union[float, torch.Tensor] = 1.0) -> None:
         """One step from the gradients as they are now."""
@@ -115,6 +144,7 @@ class AdamW:
             if gscale.dtype != torch.float32 or gscale.numel() != 1 or gscale.device != self.device:
                 raise ValueError("AdamW: gscale is a number or one fp32 value on the device of the parameters")
             gscale, dev = 1.0, gscale
+        self._stay(self._stand)
         with _on(self.device):
             rc = _native("piccl_ops_adamw_many", _STEP)(self._table.data_ptr(), self._owner.data_ptr(), self.blocks, self.bits == 8, self.m.data_ptr(), self.v.data_ptr(), _ptr(self.m_scales),
                                                         _ptr(self.v_scales), lr, b1, b2, eps, wd, gscale, _ptr(dev), self.step_dev.data_ptr(), self._ticket.data_ptr(), self.seed, _s())

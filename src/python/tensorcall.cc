@@ -5,7 +5,8 @@
 // Python function then looks at them itself and says what is wrong.
 #include <Python.h>
 #include <initializer_list>
-#include <new>
+#include <memory>
+#include <vector>
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDACachingAllocator.h>
@@ -177,18 +178,30 @@ PyObject* empty(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
-// What stays the same from step to step of an optimiser
-struct Adam { int device, bits8; long long blocks; void *table, *owner, *m, *v, *ms, *vs, *step, *ticket; unsigned seed; };
-// adamw(device, table, owner, blocks, bits8, m, v, ms, vs, step, ticket, seed), all numbers -> handle
+// What stays the same from step to step of an optimiser, and the tensors whose addresses stand in its table
+struct Adam {
+  int device, bits8; long long blocks; void *table, *owner, *m, *v, *ms, *vs, *step, *ticket; unsigned seed;
+  std::vector<at::Tensor> tensors; std::vector<const void*> places;
+};
+// adamw(device, table, owner, blocks, bits8, m, v, ms, vs, step, ticket, seed: all numbers, tuple of tensors) -> handle
 PyObject* adamw(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  long long x[12];
-  if (n != 12) { PyErr_SetString(PyExc_TypeError, "adamw: 12 numbers"); return nullptr; }
-  for (int i = 0; i < 12; i++) { x[i] = (long long)PyLong_AsUnsignedLongLongMask(a[i]); if (PyErr_Occurred()) return nullptr; }
-  auto p = [&](int i) { return reinterpret_cast<void*>(x[i]); };
-  Adam* const h = new (std::nothrow) Adam{(int)x[0], (int)x[4], x[3], p(1), p(2), p(5), p(6), p(7), p(8), p(9), p(10), (unsigned)x[11]};
-  return h ? PyCapsule_New(h, "adamw", [](PyObject* c) { delete static_cast<Adam*>(PyCapsule_GetPointer(c, "adamw")); }) : PyErr_NoMemory();
+  return guarded([&]() -> PyObject* {
+    long long x[12];
+    if (n != 13 || !PyTuple_Check(a[12])) { PyErr_SetString(PyExc_TypeError, "adamw: 12 numbers and a tuple"); return nullptr; }
+    for (int i = 0; i < 12; i++) { x[i] = (long long)PyLong_AsUnsignedLongLongMask(a[i]); if (PyErr_Occurred()) return nullptr; }
+    auto p = [&](int i) { return reinterpret_cast<void*>(x[i]); };
+    std::unique_ptr<Adam> h(new Adam{(int)x[0], (int)x[4], x[3], p(1), p(2), p(5), p(6), p(7), p(8), p(9), p(10), (unsigned)x[11], {}, {}});
+    for (Py_ssize_t i = 0; i < PyTuple_GET_SIZE(a[12]); i++) {
+      const at::Tensor* const t = tensor(PyTuple_GET_ITEM(a[12], i));
+      if (!t) { PyErr_SetString(PyExc_TypeError, "adamw: tensors wanted"); return nullptr; }
+      h->tensors.push_back(*t); h->places.push_back(t->data_ptr());
+    }
+    PyObject* const c = PyCapsule_New(h.get(), "adamw", [](PyObject* c) { delete static_cast<Adam*>(PyCapsule_GetPointer(c, "adamw")); });
+    if (c) h.release();
+    return c;
+  });
 }
-// adamw_step(handle, lr, b1, b2, eps, wd, gscale): gscale a number or a tensor; 0 if that tensor is not one fp32 value on the device
+// adamw_step(handle, lr, b1, b2, eps, wd, gscale): gscale a number or a tensor; 0 if that tensor is not one fp32 value on the device, or a tensor of the table has moved
 PyObject* adamw_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
     if (n != 7) return no();
@@ -200,6 +213,7 @@ PyObject* adamw_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (!t) { g = PyFloat_AsDouble(a[6]); if (PyErr_Occurred()) return nullptr; }
     else if (t->scalar_type() != at::kFloat || t->numel() != 1 || !t->is_cuda() || t->device().index() != h->device) return no();
     if (!(x[1] >= 0 && x[1] < 1 && x[2] >= 0 && x[2] < 1)) return no();
+    for (size_t i = 0; i < h->tensors.size(); i++) if (h->tensors[i].data_ptr() != h->places[i]) return no();
     const c10::cuda::CUDAGuard guard((c10::DeviceIndex)h->device);
     return answer(piccl_ops_adamw_many(h->table, static_cast<const int*>(h->owner), h->blocks, h->bits8, h->m, h->v, h->ms, h->vs, (float)x[0], x[1], x[2], (float)x[3], (float)x[4], (float)g,
                                        t ? t->data_ptr<float>() : nullptr, static_cast<int*>(h->step), static_cast<unsigned*>(h->ticket), h->seed, stream()), 1, "adamw_many");

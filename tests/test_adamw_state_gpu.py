@@ -146,3 +146,96 @@ def test_moments_in_32_bits_are_rounded_one_operation_at_a_time():
         opt.step(1e-3, 0.9, 0.95, 1e-8, 0.1, gscale=0.7)
         got = opt.moments(0)
         assert torch.equal(got[0], m * 0.9 + x * (1.0 - 0.9)) and torch.equal(got[1], v * 0.95 + (x * (1.0 - 0.95)) * x)
+
+
+@pytest.fixture(params=["native", "ctypes"])
+def path(request, monkeypatch):
+    """Each call path in turn (ctypes: as where Python's headers are missing)"""
+    from piccl_b200.ops import fp8
+    if request.param == "ctypes":
+        monkeypatch.setattr(fp8, "_fast", False)
+    else:
+        assert fp8._native_calls()
+    return request.param
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_the_state_cannot_part_from_the_steps(path, bits):
+    """Captured steps and the native handle have the addresses: another tensor in the place of one of these would be passed over, and what it replaced freed under the next step."""
+    from piccl_b200.ops.optimizer import AdamW
+    p, g = torch.ones(300, device="cuda"), torch.full((300,), 1e-3, device="cuda")
+    opt = AdamW([p], [g], bits=bits, seed=3)
+    opt.step(1e-3)
+    for name in ("m", "v", "m_scales", "v_scales", "step_dev", "seed", "bits", "params", "masters", "grads", "decay", "places", "blocks", "device"):
+        kept = getattr(opt, name)
+        with pytest.raises(AttributeError):
+            setattr(opt, name, kept.clone() if isinstance(kept, torch.Tensor) else kept)
+        assert getattr(opt, name) is kept or name == "seed"
+    for name in ("params", "masters", "grads", "decay", "places"):
+        assert isinstance(getattr(opt, name), tuple)
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+@pytest.mark.parametrize("where", ["cuda", "cpu"])
+def test_a_state_is_loaded_in_place(path, bits, where):
+    """An optimiser that goes on from another's state does what that one does, captured steps of its own among them."""
+    from piccl_b200.ops.optimizer import AdamW
+    sizes = [300, 0, 5, 4097]
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    start = [torch.randn(n, generator=gen, device="cuda") for n in sizes]
+    grads = [torch.randn(n, generator=gen, device="cuda") * 1e-3 for n in sizes]
+
+    def make():
+        params = [w.clone() for w in start]
+        return params, AdamW(params, grads, bits=bits, seed=7)
+
+    a, one = make()
+    for _ in range(3):
+        one.step(1e-3)
+    b, two = make()
+    graph = torch.cuda.CUDAGraph()
+    two.step(1e-3)
+    with torch.cuda.graph(graph):
+        two.step(1e-3)
+    with torch.no_grad():
+        for x, y in zip(a, b):
+            y.copy_(x)
+    two.load_state({k: t.to(where, copy=True) for k, t in one.state().items()})
+    one.step(1e-3)
+    graph.replay()
+    one.step(1e-3)
+    two.step(1e-3)
+    assert all(torch.equal(x, y) for x, y in zip(a, b)) and int(two.step_dev) == 5
+    assert all(torch.equal(t.float(), two.state()[k].float()) for k, t in one.state().items())
+    for bad in ({}, {**one.state(), "m": one.m[:128]}, {**one.state(), "v": one.v.double()}, AdamW([torch.ones(300, device="cuda")], [grads[0]], bits=40 - bits).state()):
+        with pytest.raises(ValueError):
+            two.load_state(bad)
+
+
+def test_tensors_that_have_moved_are_refused(path):
+    """A step would write where a parameter was before it was given other memory, which may be another tensor's by now."""
+    from piccl_b200.ops.optimizer import AdamW
+    def make():
+        w, p, g = torch.ones(300, device="cuda"), torch.ones(300, dtype=torch.bfloat16, device="cuda"), torch.ones(300, dtype=torch.bfloat16, device="cuda")
+        return [w, p, g], AdamW([p], [g], [w])
+    for i in range(3):
+        tensors, opt = make()
+        opt.step(1e-3)
+        old = tensors[i].data
+        tensors[i].data = tensors[i].data.clone()
+        with pytest.raises(ValueError, match="not where it was"):
+            opt.step(1e-3)
+        if i < 2:
+            with pytest.raises(ValueError, match="not where it was"):
+                opt.set_grads([tensors[2]])
+        else:
+            opt.set_grads([tensors[2]])
+            opt.step(1e-3)
+        tensors[i].data = old
+        if i == 2:
+            opt.set_grads([tensors[2]])
+        opt.step(1e-3)
+        assert int(opt.step_dev) == (3 if i == 2 else 2)
+        tensors[i].untyped_storage().resize_(0)
+        with pytest.raises((ValueError, RuntimeError)):
+            opt.step(1e-3)
