@@ -79,7 +79,21 @@ _DECAY = ("w_qkv", "w_o", "w_fc", "w_proj")
 _NODECAY = ("ln1_g", "ln1_b", "b_qkv", "b_o", "ln2_g", "ln2_b", "b_fc", "b_proj")
 
 
+def _of_the_optimizer(name: str, shared: bool) -> property:
+    """A tensor of the optimiser.  With moments in 8 bits its addresses are in ops/optimizer.py's table, so another tensor in its place would be passed over: copy into it.  shared: whether AdamW has its own."""
+    def get(self):
+        return getattr(self._adam, name) if shared and self._adam is not None else getattr(self, "_" + name)
+
+    def put(self, t):
+        if self._adam is not None:
+            raise AttributeError(f"{name} stays where it is with moments in 8 bits: copy into it")
+        setattr(self, "_" + name, t)
+    return property(get, put)
+
+
 class GPT2:
+    master, m, v, step_dev = _of_the_optimizer("master", False), _of_the_optimizer("m", True), _of_the_optimizer("v", True), _of_the_optimizer("step_dev", True)
+
     def __init__(self, cfg: GPT2Config, device="cuda", seed: int = 0, adam_bits: int = 32):
         """adam_bits: 32, or 8 for moments of the optimiser at a byte an element (ops/optimizer.py)."""
         if adam_bits not in (8, 32):
@@ -115,13 +129,12 @@ class GPT2:
             off += n
         self.n_params = total
         self._init_weights(seed)
+        self._adam = None
         self.master = self.flat_p.float()
         self.step_count = 0
-        self._adam = None
         if adam_bits == 8:
             pieces = [slice(b, e) for b, e, _ in self.groups]
             self._adam = AdamW([self.flat_p[c] for c in pieces], [self.flat_g[c] for c in pieces], [self.master[c] for c in pieces], bits=8, decay=[d for _, _, d in self.groups], seed=seed)
-            self.m, self.v, self.step_dev = self._adam.m, self._adam.v, self._adam.step_dev
         else:
             self.m = torch.zeros_like(self.master)
             self.v = torch.zeros_like(self.master)

@@ -239,3 +239,17 @@ def test_tensors_that_have_moved_are_refused(path):
         tensors[i].untyped_storage().resize_(0)
         with pytest.raises((ValueError, RuntimeError)):
             opt.step(1e-3)
+
+
+def test_gpt2_says_that_its_state_stays_where_it_is():
+    from piccl_b200.models.gpt2 import GPT2, GPT2Config
+    model = GPT2(GPT2Config.tiny(), adam_bits=8)
+    for name in ("master", "m", "v", "step_dev"):
+        with pytest.raises(AttributeError):
+            setattr(model, name, getattr(model, name).clone())
+    assert model.m is model._adam.m and model.v is model._adam.v and model.step_dev is model._adam.step_dev
+    model = GPT2(GPT2Config.tiny())          # with moments in 32 bits each step takes what is there
+    for name in ("master", "m", "v", "step_dev"):
+        other = getattr(model, name).clone()
+        setattr(model, name, other)
+        assert getattr(model, name) is other
