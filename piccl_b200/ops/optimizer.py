@@ -105,7 +105,9 @@ class AdamW:
         grads = list(grads)
         if len(grads) != len(self.params):
             raise ValueError(f"AdamW: {len(self.params)} gradients wanted, got {len(grads)}")
-        if torch.cuda.is_current_stream_capturing():
+        with _on(self.device):                        # the stream that the copy goes to
+            capturing = torch.cuda.is_current_stream_capturing()
+        if capturing:
             raise RuntimeError("AdamW: gradients cannot be exchanged within a capture")
         self._stay(self._fixed)
         records = []
