@@ -94,7 +94,7 @@ __global__ void __launch_bounds__(256, R * T <= 2 ? 2 : 1) fp8_few_kernel(const 
       for (int h = 0; h < 2; h++) {
         const int row = row0 + 16 * r + 8 * h + g;
 #pragma unroll
-        for (int c = 0; c < 2; c++) p.w[r][h][c] = row < a.N ? __ldg(reinterpret_cast<const uint4*>(a.w + row * pitch + kb * 128ll + c * 64 + t * 16)) : make_uint4(0, 0, 0, 0);
+        for (int c = 0; c < 2; c++) p.w[r][h][c] = row < a.N ? *reinterpret_cast<const uint4*>(a.w + row * pitch + kb * 128ll + c * 64 + t * 16) : make_uint4(0, 0, 0, 0);
         p.s[r][h] = row < a.N ? a.sw[scale_at(row, kb, a.k4)] : 1u;
       }
   };
@@ -185,14 +185,14 @@ __global__ void __launch_bounds__(256, 1) fp8_fragments_kernel(const FewArgs a) 
       for (int h = 0; h < 2; h++) {
         const int row = row0 + 16 * r + 8 * h + g;
 #pragma unroll
-        for (int c = 0; c < 2; c++) p.w[r][h][c] = row < a.N ? __ldg(reinterpret_cast<const uint4*>(a.w + row * pitch + kb * 128ll + c * 64 + t * 16)) : make_uint4(0, 0, 0, 0);
+        for (int c = 0; c < 2; c++) p.w[r][h][c] = row < a.N ? *reinterpret_cast<const uint4*>(a.w + row * pitch + kb * 128ll + c * 64 + t * 16) : make_uint4(0, 0, 0, 0);
         p.s[r][h] = row < a.N ? a.sw[scale_at(row, kb, a.k4)] : 1u;
       }
 #pragma unroll
     for (int n = 0; n < T; n++) {
       const int m = 8 * n + g;
 #pragma unroll
-      for (int c = 0; c < 2; c++) p.b[n][c] = m < a.M ? __ldg(reinterpret_cast<const uint4*>(a.a + m * pitch + kb * 128ll + c * 64 + t * 16)) : make_uint4(0, 0, 0, 0);
+      for (int c = 0; c < 2; c++) p.b[n][c] = m < a.M ? *reinterpret_cast<const uint4*>(a.a + m * pitch + kb * 128ll + c * 64 + t * 16) : make_uint4(0, 0, 0, 0);
 #pragma unroll
       for (int j = 0; j < 2; j++) p.f[n][j] = a.sa[scale_at(8 * n + 2 * t + j, kb, a.k4)];      // (scales have room for 128 rows)
     }

@@ -11,7 +11,8 @@ typedef __nv_bfloat16 bf16;
 // Programmatic dependent launch: the grid may start while the kernel before it on the stream still runs; what it does before
 // pdl_begin() overlaps that kernel's tail, everything after it sees the kernel before completed.  A step is hundreds of kernels of 2 to
 // 50 us, so the launch latency between two of them (1 us and more) counts.  Every kernel launched by launch_pdl calls pdl_begin()
-// before it touches global memory, reads as well as writes.
+// before it touches global memory, reads as well as writes.  (A prefetch into L2 may come before it: it is a hint, and what the kernel before writes is seen all the same.)  Loads of what a kernel before may have
+// written are plain ones: __ldg and ld.global.nc are for memory that nobody writes while the grid is there, and this one is there while that kernel still runs.
 __device__ __forceinline__ void pdl_begin() {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
