@@ -253,3 +253,22 @@ def test_gpt2_says_that_its_state_stays_where_it_is():
         other = getattr(model, name).clone()
         setattr(model, name, other)
         assert getattr(model, name) is other
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_replayed_steps_of_the_trainer_are_those_issued_one_by_one(bits):
+    """Losses, weights and the optimiser's state, bit for bit: a replay goes on counting and draws other random bits than the capture."""
+    from piccl_b200.models.gpt2 import GPT2Config
+    from piccl_b200.train import DataParallelTrainer
+    cfg = GPT2Config.tiny()
+    tok = torch.randint(0, cfg.vocab_size, (6, 2, cfg.seq_len + 1), generator=torch.Generator().manual_seed(0))
+    runs = []
+    for graph in (False, True):
+        tr = DataParallelTrainer(cfg, None, seed=3, adam_bits=bits, use_graph=graph)
+        losses = [tr.step(t[:, :-1].contiguous().pin_memory(), t[:, 1:].contiguous().pin_memory()) for t in tok]
+        state = tr.model._adam.state() if bits == 8 else {"m": tr.model.m, "v": tr.model.v, "step_dev": tr.model.step_dev}
+        assert tr.replayed_steps() >= 3 if graph else True
+        runs.append((losses, {"master": tr.model.master, "p": tr.model.flat_p, **state}))
+    assert runs[0][0] == runs[1][0]
+    for name, t in runs[0][1].items():
+        assert torch.equal(t.float(), runs[1][1][name].float()), name
