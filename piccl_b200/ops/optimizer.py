@@ -9,7 +9,12 @@ step can be captured into a CUDA graph and replayed; `gscale` multiplies the gra
 
 Moments are the optimiser's own: `m` and `v`, flat, each tensor from a multiple of 128 elements on (`places`).  In 8 bits they are e4m3 values with
 a power of two for each block of 128 (`m_scales`, `v_scales`: byte e stands for 2^(e - 127)), v as its root, and are rounded stochastically, by bits that
-depend on the element's place, the step and `seed` alone: 2.02 bytes a parameter in place of 8.  Values that are not finite are held as NaN.
+depend on the element's place, the step and `seed` alone: 2.02 bytes a parameter in place of 8 (and 0.03 for the table that tells each block's tensor).  Values that are not finite are held as NaN.
+
+What 8 bits cost: each held value is within a step of e4m3 (6 to 12 %) of the one that it stands for, and right in the mean.  The square of a root that is right in the mean is too large by the rounding's
+variance: at most 13.5 % in the mean of v, 2.5 % measured at b2 = 0.95 and 3.4 % at 0.999 (gradients of one size); an element's root has a deviation of 12 to 16 %, 98 % of them are between 0.73 and 1.4 times the exact one.  The random bits
+of a place at one step are those of the place after it at the step before: an element's own roundings are independent from step to step, but the errors of neighbours' roots go together (correlation 0.3 to 0.46 from
+one element to the next, over some 1 / (1 - b2) elements; none in m, where signs differ).
 These tensors, `step_dev` and `seed` are what captured steps go on reading and cannot be exchanged: a state is loaded into them (`load_state`, or `opt.m.copy_(...)`).  Parameters, masters and gradients stay where
 they are too; a step after one of them has been given other memory (`p.data = ...`) is refused.
 

@@ -272,3 +272,27 @@ def test_replayed_steps_of_the_trainer_are_those_issued_one_by_one(bits):
     assert runs[0][0] == runs[1][0]
     for name, t in runs[0][1].items():
         assert torch.equal(t.float(), runs[1][1][name].float()), name
+
+
+@pytest.mark.parametrize("b2,steps", [(0.95, 1000), (0.99, 2000), (0.999, 4000)])
+def test_how_far_second_moments_in_8_bits_are_too_large(b2, steps):
+    """The root is rounded without bias, so its square is too large by the rounding's variance.  A root r that would move by d is rounded up with the probability d / s of its step s, a variance of at most |d| s, with
+    |d| <= (1 - b2) |g^2 - r^2| / (r (1 + sqrt b2)) and s <= r / 8.  In the mean V of the squares, k = 1 / (8 (1 + sqrt b2)): V <= b2 V + (1 - b2) (G + k (G + V)), so G <= V <= G (1 + k) / (1 - k), at any step.
+    Of n elements the mean is off by no more than eight of its deviations, counted as if 2 / (1 - b2) neighbours went together, the steps that a moment remembers (a place's bits at a step are those of the place after it at
+    the step before)."""
+    from piccl_b200.ops.optimizer import AdamW
+    n = 1 << 20
+    gen = torch.Generator(device="cuda").manual_seed(11)
+    g = torch.empty(n, device="cuda")
+    eight, full = (AdamW([torch.zeros(n, device="cuda")], [g], bits=bits, seed=1) for bits in (8, 32))
+    for _ in range(steps):
+        g.normal_(generator=gen)
+        for o in (eight, full):
+            o.step(0.0, 0.9, b2, 1e-8, 0.0)
+    (m8, v8), (m32, v32) = (tuple(t.double() for t in o.moments(0)) for o in (eight, full))
+    k, far = 1 / (8 * (1 + math.sqrt(b2))), 8 / math.sqrt(n * (1 - b2) / 2)
+    ratio, spread = float(v8.mean() / v32.mean()), float((v8 / v32).std())
+    print("mean", ratio, "deviation of one", spread)
+    assert 1 - far * spread <= ratio <= (1 + k) / (1 - k) + far * spread
+    # the first moment has no bias: its mean is that of the exact one within the same count
+    assert abs(float((m8 - m32).mean())) <= 8 / math.sqrt(n * 0.1 / 2) * float((m8 - m32).std())
