@@ -12,8 +12,8 @@ dimensions is kept twice, the second time transposed; `square` gives both copies
     fp8.linear_bwd(dy, xt, w8t, dx, dw)                      # dx = dy w, dw = dy^T x
 
 Sums are fp32 in the tensor cores, which cut off where an fma would round: each step of 32 k loses up to 2^-23 of the sum so far, always toward zero.  Results in fp32 are added up, rounded, from sums of 1024 k;
-those in bf16 are one sum over all of k, which over K values of one sign is too small by up to 2^-23 K / 64 of it (measured 2^-25 K / 48 of the sum of magnitudes with random signs: 5e-6 at K = 8192,
-beside the 2e-3 of a rounding to bf16).  Results are rounded once.  Calls launch on the current stream of their tensors' device, take workspace from PyTorch's
+those in bf16 are one sum over all of k, which is too small by up to 2^-23 K / 64 of it where all addends have one sign (1.5e-5 at K = 8192, beside the 2e-3 of a rounding to bf16), and with random signs by some
+2^-25 K / 48 of a result's usual size.  Results are rounded once.  Calls launch on the current stream of their tensors' device, take workspace from PyTorch's
 allocator, and can be captured.  Results overlap neither operands nor each other.  Empty results are left alone; a sum over nothing is zero (or the bias).
 """
 from __future__ import annotations
