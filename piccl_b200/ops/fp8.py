@@ -178,10 +178,10 @@ def linear(x: torch.Tensor, w: Fp8, out: torch.Tensor, bias: Optional[torch.Tens
     _check_apart("linear", [out, *(keep or ())], [x, *w, bias])
     if w.values.dim() != 2 or w.values.shape[1] != (K + 127) // 128 * 128:
         raise ValueError(f"linear: weights of {K} columns wanted, got {tuple(w.values.shape)}")
+    _check_product((M, w.values.shape[1]), w, out, bias)          # all of it before anything is written
+    if out.device != x.device:
+        raise ValueError("linear: tensors of one CUDA device wanted")
     if keep is None and M and K and M <= 64 and not _native("piccl_ops_fp8_linear_scratch", _SCRATCH)(x.data_ptr(), x.dtype == torch.float32, x.stride(0) if M > 1 else K, M, w.values.shape[0], K, False):
-        _check_product((M, w.values.shape[1]), w, out, bias)
-        if out.device != x.device:
-            raise ValueError("linear: tensors of one CUDA device wanted")
         if out.numel() == 0:
             return out
         with _on(x.device):
@@ -211,6 +211,11 @@ def linear_bwd(dy: torch.Tensor, xt: Optional[Fp8], wt: Optional[Fp8], dx: Optio
     for a, n in ((wt if dx is not None else None, Nn), (xt if dw is not None else None, M)):
         if a is not None and (a.values.dim() != 2 or a.values.shape[1] != (n + 127) // 128 * 128):
             raise ValueError(f"linear_bwd: {n} columns wanted, got {tuple(a.values.shape)}")
+    for b, out, rows in ((wt, dx, M), (xt, dw, Nn)):
+        if out is not None:                                           # all of it before anything is written
+            _check_product((rows, b.values.shape[1]), b, out, None)
+            if out.device != dy.device:
+                raise ValueError("linear_bwd: tensors of one CUDA device wanted")
     q = empty(M, Nn, dy.device) if dx is not None else None
     t = empty(Nn, M, dy.device) if dw is not None else None
     quantize(dy, q, t)

@@ -54,3 +54,24 @@ def test_out_of_memory_is_pytorchs_own_error(path):
     fp8.quantize(x, q)
     want = fp8.product(q, w, torch.empty_like(y))
     assert torch.equal(y, want)
+
+
+def test_refused_calls_write_nothing(path):
+    """A call with one argument that is not as it has to be leaves the others alone, whichever it is."""
+    from piccl_b200.ops import fp8
+    M, N, K = 40, 72, 264
+    x, dy, w, wt, xt = _randn(M, K), _randn(M, N), fp8.empty(N, K), fp8.empty(K, N), fp8.empty(K, M)
+    fp8.quantize(_randn(N, K, seed=1), w, transposed=wt, square=True)
+    fp8.quantize(x, None, transposed=xt)
+    y, dx, dw = (torch.full(s, 7.0, dtype=torch.bfloat16, device="cuda") for s in ((M, N), (M, K), (N, K)))
+    keep = fp8.empty(K, M)
+    keep.values.view(torch.uint8).fill_(5)
+    keep.scales.fill_(9)
+    bias = _randn(N)
+    for call in (lambda: fp8.linear(x, w, y, bias=bias[:9], keep=keep), lambda: fp8.linear(x, w, y.half(), keep=keep), lambda: fp8.linear(x, w, y[:9], keep=keep), lambda: fp8.linear(x, w, y.cpu(), keep=keep),
+                 lambda: fp8.linear(x, fp8.Fp8(w.values, w.scales[:0]), y, keep=keep), lambda: fp8.linear(x, w, y, bias=bias.cpu(), keep=keep), lambda: fp8.linear(x, w, y, keep=fp8.Fp8(keep.values, keep.scales[:1])),
+                 lambda: fp8.linear_bwd(dy, xt, wt, dx, dw.half()), lambda: fp8.linear_bwd(dy, xt, wt, dx, dw[:9]), lambda: fp8.linear_bwd(dy, xt, wt, dx, dw.cpu()), lambda: fp8.linear_bwd(dy, xt, wt, dx.t(), dw),
+                 lambda: fp8.linear_bwd(dy, fp8.Fp8(xt.values, xt.scales[:1]), wt, dx, dw), lambda: fp8.linear_bwd(dy, xt, fp8.Fp8(wt.values.view(torch.uint8), wt.scales), dx, dw)):
+        with pytest.raises(ValueError):
+            call()
+        assert all(bool((t == 7.0).all()) for t in (y, dx, dw)) and bool((keep.values.view(torch.uint8) == 5).all()) and bool((keep.scales == 9).all())
