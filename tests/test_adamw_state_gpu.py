@@ -296,3 +296,20 @@ def test_how_far_second_moments_in_8_bits_are_too_large(b2, steps):
     assert 1 - far * spread <= ratio <= (1 + k) / (1 - k) + far * spread
     # the first moment has no bias: its mean is that of the exact one within the same count
     assert abs(float((m8 - m32).mean())) <= 8 / math.sqrt(n * 0.1 / 2) * float((m8 - m32).std())
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+@pytest.mark.parametrize("factor", [math.inf, math.nan])
+def test_what_lies_between_tensors_stays_zero(bits, factor):
+    """Also where the factor of the gradients is not finite, which makes NaN of every moment that is a tensor's: moments loaded over them are whole again, and a norm over the flat state is the tensors'."""
+    from piccl_b200.ops.optimizer import AdamW
+    sizes = [1, 130, 7, 256, 1001]
+    params, grads = [torch.ones(n, device="cuda") for n in sizes], [torch.full((n,), 1e-3, device="cuda") for n in sizes]
+    opt = AdamW(params, grads, bits=bits)
+    opt.step(1e-3)
+    opt.step(1e-3, gscale=torch.full((1,), factor, device="cuda"))
+    inside = torch.zeros(opt.m.numel(), dtype=torch.bool, device="cuda")
+    for o, n in opt.places:
+        inside[o:o + n] = True
+    for t in (opt.m.float(), opt.v.float()):
+        assert bool((t[~inside] == 0).all()) and not bool(t[inside].isfinite().any())
