@@ -181,7 +181,7 @@ def linear(x: torch.Tensor, w: Fp8, out: torch.Tensor, bias: Optional[torch.Tens
     _check_product((M, w.values.shape[1]), w, out, bias)          # all of it before anything is written
     if out.device != x.device:
         raise ValueError("linear: tensors of one CUDA device wanted")
-    if keep is None and M and K and M <= 64 and not _native("piccl_ops_fp8_linear_scratch", _SCRATCH)(x.data_ptr(), x.dtype == torch.float32, x.stride(0) if M > 1 else K, M, w.values.shape[0], K, False):
+    if keep is None and K and 0 < M <= 32 and not _native("piccl_ops_fp8_linear_scratch", _SCRATCH)(x.data_ptr(), x.dtype == torch.float32, x.stride(0) if M > 1 else K, M, w.values.shape[0], K, False):
         if out.numel() == 0:
             return out
         with _on(x.device):

@@ -1,4 +1,4 @@
-// The instructions of products in the format of fp8.cuh: tcgen05.mma kind::mxf8f6f4 on one CTA or a pair, and the tensor maps of their operands.
+// The instructions of products in the format of fp8.cuh: tcgen05.mma kind::mxf8f6f4 on a pair of CTAs, and the tensor maps of their operands.
 #pragma once
 #include "../include/sm100_gemm_pair.cuh"
 
@@ -17,18 +17,6 @@ __device__ __forceinline__ void scales_to_tmem_pair(uint32_t taddr, uint64_t des
 __device__ __forceinline__ void umma_mxf8_pair(uint32_t tmem_d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t sfa, uint32_t sfb, uint32_t accumulate) {
   asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\ttcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}\n"
                ::"r"(tmem_d), "l"(da), "l"(db), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate) : "memory");
-}
-// one CTA
-__device__ __forceinline__ void scales_to_tmem(uint32_t taddr, uint64_t desc) {
-  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
-}
-__device__ __forceinline__ void umma_mxf8(uint32_t tmem_d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t sfa, uint32_t sfb, uint32_t accumulate) {
-  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\ttcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}\n"
-               ::"r"(tmem_d), "l"(da), "l"(db), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate) : "memory");
-}
-__device__ __forceinline__ void tma_load_2d(void* smem_dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
-  asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
-               ::"r"(smem_u32(smem_dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y) : "memory");
 }
 
 // [rows, cols] of elements of esz bytes (1: e4m3, 2: bf16, 4: fp32 or words of scales), boxes of box_rows x box_cols; swizzle: of rows of 128 bytes

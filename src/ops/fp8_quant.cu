@@ -54,7 +54,7 @@ __global__ void __launch_bounds__(256) quant_rows_kernel(const QuantArgs a) {
 
 // A block has a tile of 128 x 128 in registers as it came, a thread 8 x 8 of it (16 lanes beside each other to a row).  The largest magnitudes of its rows and columns go through shared memory
 // at one barrier; half of the threads then put the rows' together, half the columns'.  (The rows' by shuffles, 32 a thread: 42 us for
-// 8192 x 4096 bf16 both ways, in place of 26.5.)  Bound by the latencies of loads and barriers at 17 instructions a value, 5.1 TB/s; four blocks to an SM, at 64 registers and a spill of two, take 26.5 us where three take 27.2.
+// 8192 x 4096 bf16 both ways, in place of 26.5.)  Bound by the latencies of loads and barriers at 17 instructions a value, 5.1 TB/s; four blocks to an SM, at 64 registers and a spill of 16 bytes (28 stored and 56 loaded where rows are read value by value), take 26.5 us where three take 27.2.
 // Magnitudes of the two kinds: 128 lines of 16 partial maxima, a line's partial i at [i][line], and every [i] moved on by 16 bytes so that threads side by side do not meet in a bank.
 template <typename T> struct Tops {
   static constexpr int PITCH = 128 * sizeof(T) + 16;       // bf16: 16 bits each
@@ -233,7 +233,7 @@ using namespace piccl_ops;
 extern "C" {
 
 // x: [R, C], rows `stride` elements apart; fp32: float, else bf16.  q [R][C up to 128] with scales qs and t [C][R up to 128] with scales ts: either pair may be null, not both.
-// q, t: 8-byte aligned or better; qs, ts: 4-byte aligned.
+// x at any element's address; q, qs, t and ts on 16-byte boundaries.
 int piccl_ops_fp8_quantize(const void* x, int fp32, long long R, long long C, long long stride, void* q, void* qs, void* t, void* ts, int square, void* stream) {
   if (R <= 0 || C <= 0 || R > 0x7fffff00ll || C > 0x7fffff00ll || stride < C) return -1;
   if (!x || (!q && !t) || !q != !qs || !t != !ts) return -2;
