@@ -34,8 +34,7 @@ __device__ __forceinline__ f32x2 sum2_alone(f32x2 a, f32x2 b, float one) { retur
 __device__ __forceinline__ uint32_t random_bits(uint32_t place, uint32_t key) {
   uint32_t h = place * 0x9E3779B9u + key;      // the golden ratio, then the roots of 3 and 2: odd numbers without a pattern
   h = (h ^ (h >> 16)) * 0xBB67AE85u;
-  h = (h ^ (h >> 15)) * 0x6A09E667u;
-  return h ^ (h >> 16);
+  return (h ^ (h >> 15)) * 0x6A09E667u;
 }
 __device__ __forceinline__ void e4m3_values(uint32_t four, float f, f32x2 (&v)[2]) {      // times f
 #pragma unroll
@@ -47,17 +46,17 @@ __device__ __forceinline__ void e4m3_values(uint32_t four, float f, f32x2 (&v)[2
 }
 __device__ __forceinline__ float max3_nan(float a, float b, float c) { float r; asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c)); return r; }
 __device__ __forceinline__ float min3(float a, float b, float c) { float r; asm("min.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c)); return r; }
-// Where an element's 16 random bits stand among the 20 that are cut off
-template <bool ROOT> __device__ __forceinline__ uint32_t random_part(uint32_t r) { return (ROOT ? r >> 16 : r & 0xffffu) << 4; }
+// An element's 16 random bits, of h ^ (h >> 16): the upper half for the root, the lower one for m
+template <bool ROOT> __device__ __forceinline__ uint32_t random_part(uint32_t h) { return ROOT ? h >> 16 : (h ^ h >> 16) & 0xffffu; }
 // x / scale, at most 448 in magnitude, rounded: what is cut off of its fraction, and the random bits, carry.  Its magnitude is 2^-6 or more: the steps of e4m3 are those of three bits of fraction.
-template <bool ROOT> __device__ __forceinline__ float stochastic(float t, uint32_t r) { return __uint_as_float((__float_as_uint(t) + random_part<ROOT>(r)) & 0xfff00000u); }
-// The same for any magnitude, and NaN for x that is not finite; a root that is not zero stays so
-template <bool ROOT> __device__ __forceinline__ float stochastic_any(float x, float t, uint32_t r) {
-  if ((__float_as_uint(x) & 0x7fffffffu) >= kInf) return __uint_as_float(0x7fffffffu);
+template <bool ROOT> __device__ __forceinline__ float stochastic(float t, uint32_t r) { return __uint_as_float((__float_as_uint(t) + (random_part<ROOT>(r) << 4)) & 0xfff00000u); }
+// The same for any magnitude, and NaN for x that is not finite; a root that is not zero stays so.  sum: whose upper bits are taken
+template <bool ROOT> __device__ __forceinline__ float stochastic_any(float x, float t, uint32_t r, uint32_t& sum) {
   const float a = fabsf(t), low = a < 0.015625f ? 0.015625f : 0.f;      // below 2^-6 the steps are those of [2^-6, 2^-5)
-  float z = stochastic<ROOT>(a + low, r) - low;
+  sum = __float_as_uint(a + low) + (random_part<ROOT>(r) << 4);
+  float z = __uint_as_float(sum & 0xfff00000u) - low;
   if (ROOT && a > 0.f) z = fmaxf(z, 0.001953125f);
-  return copysignf(z, t);
+  return (__float_as_uint(x) & 0x7fffffffu) >= kInf ? __uint_as_float(0x7fffffffu) : copysignf(z, t);
 }
 // The byte of a block whose largest value is the root of v: the smallest s for which v <= (448 * 2^s)^2 = 1.53125 * 2^(17 + 2 s).  (A root rounded to fp32 is above 448 * 2^s exactly
 // where v is above that, so this is the byte of correctly rounded roots.)
@@ -72,8 +71,8 @@ __device__ __forceinline__ uint2 e4m3_bytes(const float (&t)[8]) {
 // Eight moments and roots of a block, by 16 lanes -> their bytes and the block's two.  All lanes of a warp call it together (votes and shuffles among a part of them cost a barrier each), and both
 // maxima are found side by side: one after the other, each behind its own votes, the latencies of shuffles were a third of the kernel's time.
 // What is held is the correctly rounded root's: whether the random bits carry can hang on its last bit, and a carry is a whole step of e4m3.  r2 are approximate roots, off by less than four units in the last place (2^-23 is
-// two, and half a one is the rounding), so they decide where the sum is at least that far from a carry.  Nearer ones, eight in 2^20, and whatever is below 2^-6, are rounded again from roots by
-// __fsqrt_rn: GPT-2 medium 1166 us (1111 with approximate roots alone, 1220 with __fsqrt_rn throughout; 1178 with the random bits kept for the second rounding).
+// two, and half a one is the rounding), so they decide where the sum is at least that far from a carry.  The nearer ones, eight in 2^20, are rounded again from roots by __fsqrt_rn: GPT-2 medium 1178 us, the smallest
+// model 8.5 (1137 and 8.5 with approximate roots alone; 1202 and 9.4 with __fsqrt_rn for whatever is below 2^-6 too; 1220 and 9.2 with it throughout).
 __device__ __forceinline__ void round_moments(const f32x2 (&m2)[4], const f32x2 (&v2)[4], const f32x2 (&r2)[4], float r_least, uint32_t place, uint32_t key, uint2& m_out, uint2& v_out, uint32_t& m_byte, uint32_t& v_byte) {
   float m[8], v[8];
 #pragma unroll
@@ -105,28 +104,25 @@ __device__ __forceinline__ void round_moments(const f32x2 (&m2)[4], const f32x2 
   float a[8], b[8];
 #pragma unroll
   for (int i = 0; i < 4; i++) { unpack2(mul2(m2[i], both2(fm)), a[2 * i], a[2 * i + 1]); unpack2(mul2(r2[i], both2(fr)), b[2 * i], b[2 * i + 1]); }
+  uint32_t sum[8];                                          // of roots and random bits: the low 20 are cut off
   if (odd) {
 #pragma unroll
-    for (int e = 0; e < 8; e++) a[e] = stochastic_any<false>(m[e], a[e], random[e]);
+    for (int e = 0; e < 8; e++) { uint32_t none; a[e] = stochastic_any<false>(m[e], a[e], random[e], none); b[e] = stochastic_any<true>(v[e], b[e], random[e], sum[e]); }
   } else {
-    uint32_t near = 0xffffffffu;                            // the low 20 bits of the sums, as distances from four below a carry
 #pragma unroll
-    for (int e = 0; e < 8; e += 2) {
-      uint32_t sum[2];
-#pragma unroll
-      for (int i = 0; i < 2; i++) {
-        a[e + i] = stochastic<false>(a[e + i], random[e + i]);
-        sum[i] = __float_as_uint(b[e + i]) + random_part<true>(random[e + i]) + 4u;
-        b[e + i] = __uint_as_float(sum[i] & 0xfff00000u);
-      }
-      near = __vimin3_u32(near, sum[0] << 12, sum[1] << 12);
+    for (int e = 0; e < 8; e++) {
+      a[e] = stochastic<false>(a[e], random[e]);
+      sum[e] = __float_as_uint(b[e]) + (random_part<true>(random[e]) << 4);
+      b[e] = __uint_as_float(sum[e] & 0xfff00000u);
     }
-    odd = __any_sync(0xffffffffu, near < 8u << 12);
   }
-  if (odd) {
+  uint32_t near = 0xffffffffu;
+#pragma unroll
+  for (int e = 0; e < 8; e += 2) near = __vimin3_u32(near, (sum[e] << 12) + (4u << 12), (sum[e + 1] << 12) + (4u << 12));
+  if (__any_sync(0xffffffffu, near < 8u << 12)) {
     asm volatile("" : "+r"(place));                         // the bits are computed again, not kept
 #pragma unroll
-    for (int e = 0; e < 8; e++) { const float root = __fsqrt_rn(v[e]); b[e] = stochastic_any<true>(root, root * fr, random_bits(place + e, key)); }
+    for (int e = 0; e < 8; e++) { const float root = __fsqrt_rn(v[e]); uint32_t none; b[e] = stochastic_any<true>(root, root * fr, random_bits(place + e, key), none); }
   }
   m_out = e4m3_bytes(a); v_out = e4m3_bytes(b);
 }
@@ -194,11 +190,11 @@ struct AdamStep {
       if (BITS8) least = k ? min3(least, x, y) : fminf(x, y);
       root[k] = pack2(x, y);
     }
-    if (BITS8 && least == 0.f) {                            // zero, or below 2^-126, where the approximate root is zero
+    if (BITS8 && least == 0.f) {                            // v is zero, or below 2^-126: the root of it times 2^64
 #pragma unroll
       for (int k = 0; k < E / 2; k++) {
         float x, y, p, q; unpack2(v[k], x, y); unpack2(root[k], p, q);
-        root[k] = pack2(p == 0.f ? __fsqrt_rn(x) : p, q == 0.f ? __fsqrt_rn(y) : q);
+        root[k] = pack2(p == 0.f ? adam_root<true>(x * 0x1p64f) * 0x1p-32f : p, q == 0.f ? adam_root<true>(y * 0x1p64f) * 0x1p-32f : q);
       }
     }
 #pragma unroll
@@ -281,7 +277,7 @@ __global__ void __launch_bounds__(256, 3) adamw_many_kernel(const AdamArgs a) {
 }
 
 // Moments in 8 bits: a lane has eight elements, sixteen lanes a block, a warp two blocks.  16 bytes an element (868 us of memory for GPT-2 medium) and about as much arithmetic: two roundings, a root and a division each.
-// 1166 us there, 4.9 TB/s; before the held roots were rounded correctly 1111, without the prefetch of the next block's lines 1245, with 16 warps to an SM in place of 24 1395.
+// 1178 us there, 4.8 TB/s; before the held roots were rounded correctly 1111, without the prefetch of the next block's lines 1245, with 16 warps to an SM in place of 24 1395.
 __global__ void __launch_bounds__(256, 3) adamw_many8_kernel(const AdamArgs a) {
   constexpr int E = 8;
   pdl_begin();
